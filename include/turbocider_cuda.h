@@ -434,6 +434,136 @@ int tc_cuda_weight_load_gguf(tc_cuda_ctx *ctx, const tc_gguf *file, uint64_t ind
 /* Validate a split set (validate_split_set, gguf_directory.hpp:273-304). */
 int tc_gguf_validate_split(const tc_gguf *const *shards, uint32_t n);
 
+/* ------------------------------------- between the projections: attention
+ * What stands between a block's query / key / value projection and its output
+ * projection: the norm and position rotation of queries and keys, appending
+ * keys and values to a paged cache, and attention of the new tokens over that
+ * cache.  (The reference runs these as separate MLX array operations around
+ * its linears, native/models/qwen21/transformer.cpp:857-953.)  All pointers
+ * are device pointers; strides count elements; sums, norms, angles and the
+ * softmax are fp32 or wider and every result is rounded once to its type.
+ * Indices read from device memory (offsets, lengths, page numbers) are
+ * checked there: an impossible one sets TC_STATUS_GEOMETRY and is skipped.
+ */
+
+/* Heads of one projection, as a [n_tokens][n_heads][head_dim] view.  `weight`
+ * (f32 [head_dim], NULL = ones) is the norm's.  `out` may be `x` itself. */
+typedef struct tc_heads {
+    const void *x;
+    void *out;
+    const float *weight;
+    uint64_t ld_token, ld_head, ld_out_token, ld_out_head;
+    uint32_t n_heads;
+    uint32_t reserved;           /* 0 */
+} tc_heads;
+
+/* Position rotation.  Pair i of a head turns by positions[token][axis(i)] *
+ * freq[i] radians and is scaled by `amplitude`:
+ *   (a, b) -> amplitude * (a cos - b sin, b cos + a sin)
+ * with (a, b) = (x[i], x[i + rotary_dim / 2]) for TC_ROPE_HALF and
+ * (x[2i], x[2i + 1]) for TC_ROPE_INTERLEAVED; elements from rotary_dim on pass
+ * through.  With n_axes > 1 (image tokens: frame, row, column) the first
+ * sections[0] pairs follow axis 0, the next sections[1] axis 1, and so on
+ * (their sum is rotary_dim / 2).  freq is f64 and the angle is formed in
+ * 64-bit fixed point modulo one turn, so it is exact to fp32 at every int32
+ * position.  positions NULL (tc_cuda_kv_append only, n_axes 1): each token's
+ * position in its cache. */
+enum { TC_ROPE_HALF = 0, TC_ROPE_INTERLEAVED = 1 };
+typedef struct tc_rope {
+    const double *freq;          /* [rotary_dim / 2] */
+    const int32_t *positions;    /* [n_tokens][n_axes], contiguous */
+    uint32_t rotary_dim, layout, n_axes;
+    uint32_t sections[4];
+    float amplitude;
+} tc_rope;
+
+/* Frequencies (host memory, rotary_dim / 2 of them) of a rotation with base
+ * theta, and the amplitude that goes with them, scaled for contexts `factor`
+ * times the trained one (trained_length):
+ *   TC_ROPE_PLAIN    theta^(-2i / rotary_dim)
+ *   TC_ROPE_LINEAR   divided by factor
+ *   TC_ROPE_NTK      theta raised to theta * factor^(d / (d - 2)), d = rotary_dim
+ *   TC_ROPE_YARN     pairs that turn more than beta_fast times in
+ *                    trained_length kept, fewer than beta_slow divided by
+ *                    factor, linear in the pair index between; amplitude
+ *                    0.1 ln(factor) + 1
+ *   TC_ROPE_BANDS    as above with beta_fast / beta_slow turns, but blended
+ *                    linearly in the number of turns; amplitude 1 */
+enum { TC_ROPE_PLAIN = 0, TC_ROPE_LINEAR = 1, TC_ROPE_NTK = 2, TC_ROPE_YARN = 3, TC_ROPE_BANDS = 4 };
+int tc_rope_freqs(uint32_t rotary_dim, double theta, uint32_t scaling, double factor, double trained_length,
+                  double beta_fast, double beta_slow, double *freq, float *amplitude);
+
+/* y = rotate(x * rsqrt(mean(x^2) + eps) * weight) for every head of q and of k
+ * (NULL: none) in one launch.  rms_norm 0: rotation only; rope NULL: norm
+ * only.  dtype f32, f16 or bf16; head_dim a multiple of 8, at most 256;
+ * rotary_dim a multiple of 8, at most head_dim. */
+int tc_cuda_qk_norm_rope(tc_cuda_ctx *ctx, const tc_heads *q, const tc_heads *k, uint64_t n_tokens,
+                         uint32_t head_dim, int dtype, int rms_norm, float eps, const tc_rope *rope,
+                         void *stream);
+
+/* A cache of keys and values in pages of page_size tokens (a power of two, 8
+ * to 65536): element (page, head, token, d) of both at page * ld_page + head *
+ * ld_head + token * ld_token + d.  dtype f16 or bf16; head_dim a multiple of
+ * 8, at most 256; k and v 16-byte aligned, strides multiples of 8. */
+typedef struct tc_paged_cache {
+    void *k, *v;
+    uint64_t ld_page, ld_head, ld_token;
+    uint32_t n_pages, page_size, n_heads, head_dim, dtype;
+    uint32_t reserved;           /* 0 */
+} tc_paged_cache;
+
+/* A step: the new tokens of n_seq requests, packed one after the other
+ * (request b has tokens new_offsets[b] .. new_offsets[b + 1] - 1, possibly
+ * none), and where their caches lie.  lengths[b] counts the request's cached
+ * tokens, the new ones included, so the new ones take its last places;
+ * entry j of its row of page_table (table_width entries, row stride ld_table)
+ * is the page of its tokens j * page_size onward.  A request of length 0 (an
+ * unused place of a fixed-size batch) caches and attends nothing.  Tokens from
+ * new_offsets[n_seq] on belong to no request and are left alone.  max_new and
+ * max_length bound the values in device memory (a request beyond them sets
+ * TC_STATUS_GEOMETRY and is treated as having length 0, with no row past
+ * max_new written); the launch is sized by them. */
+typedef struct tc_paged_batch {
+    const int32_t *new_offsets;  /* [n_seq + 1] */
+    const int32_t *lengths;      /* [n_seq] */
+    const int32_t *page_table;   /* [n_seq][ld_table] */
+    uint32_t n_seq, table_width, ld_table;
+    uint32_t n_tokens, max_new, max_length;
+} tc_paged_batch;
+
+/* Writes the new tokens' keys (normed and rotated as in tc_cuda_qk_norm_rope;
+ * rms_norm 0 and rope NULL leave them as they are) and values to the cache,
+ * and norms and rotates the queries q -> q->out (NULL: none), in one launch.
+ * k->out and v->out are not used.  The norm and rotation apply to k and q. */
+int tc_cuda_kv_append(tc_cuda_ctx *ctx, const tc_paged_cache *cache, const tc_paged_batch *batch,
+                      const tc_heads *k, const tc_heads *v, const tc_heads *q, int rms_norm, float eps,
+                      const tc_rope *rope, void *stream);
+
+/* out = softmax(scale * q K^T) V over each request's cache, for every new
+ * token and query head; query head h reads cache head h / (n_heads /
+ * cache->n_heads).  A new token at cache position p sees the positions j of
+ * its request's cache with
+ *   causal:  j <= p, and j > p - window  where window > 0;
+ *   else:    all,    and |j - p| < window where window > 0.
+ * A row that sees nothing gives zeros (lse -inf).  q and out are
+ * [n_tokens][n_heads][head_dim] of the cache's dtype; lse (NULL: none) is f32
+ * [n_tokens][n_heads], the natural log of the sum of exp(scale q k).  A NaN or
+ * infinity in a cached value that a row does not see may still reach rows of
+ * the same request; past the request's length nothing is read into results.
+ * Long caches are split over CTAs with partial results in the context's
+ * workspace. */
+typedef struct tc_attention {
+    const void *q;
+    void *out;
+    float *lse;
+    uint64_t ld_q_token, ld_q_head, ld_out_token, ld_out_head;
+    uint32_t n_heads;
+    int32_t causal, window;
+    float scale;
+} tc_attention;
+int tc_cuda_paged_attention(tc_cuda_ctx *ctx, const tc_paged_cache *cache, const tc_paged_batch *batch,
+                            const tc_attention *attention, void *stream);
+
 /* Host-side GGUF K-quant quantiser (not in the reference, which ships no
  * encoder): quantise a row-major fp32 [rows, cols] matrix (cols % 256 == 0) to
  * raw GGUF blocks of `ggml_type` (Q4_K or Q6_K) using `threads` CPU threads.

@@ -1,0 +1,85 @@
+// Shared pieces of the attention operators (attn_heads.cu, attn_paged.cu,
+// attn_chunk_sm100.cu): views of the paged cache and of a step's batch, the
+// checks of what is read from device memory, and host-side argument checks.
+#pragma once
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+#include "../../include/turbocider_cuda.h"
+#include "tc_internal.h"
+
+namespace tc {
+
+constexpr uint32_t kStatusGeometry = 1u << 3;
+constexpr int32_t kMaxLength = 1 << 30;   // cached tokens of one request (sums with a window stay in int32)
+
+// The step of tc_paged_batch, as kernels read it.
+struct BatchView {
+    const int32_t *new_offsets, *lengths, *page_table;
+    uint32_t n_seq, table_width, ld_table, n_tokens, max_new, max_length;
+};
+
+struct CacheView {
+    uint16_t *k, *v;
+    uint64_t ld_page, ld_head, ld_token;
+    uint32_t n_pages, page_size, page_shift, n_heads, head_dim;
+};
+
+// One request of the step.  length < 0: nothing of it can be used (its
+// values in device memory are impossible).
+struct Request {
+    int32_t first, n_new, length;   // first row of q, new tokens, cached tokens
+};
+
+#ifdef __CUDACC__
+// Request b with its values checked: rows inside q, a length that its row of
+// the page table covers, nothing past the bounds the launch was sized by.
+__device__ __forceinline__ Request load_request(const BatchView &bt, uint32_t page_shift, uint32_t b,
+                                                uint32_t *status) {
+    Request r;
+    r.first = bt.new_offsets[b];
+    const int32_t end = bt.new_offsets[b + 1];
+    r.length = bt.lengths[b];
+    if (r.first < 0 || end < r.first || (uint32_t)end > bt.n_tokens) {
+        atomicOr(status, kStatusGeometry);
+        return Request{0, 0, 0};
+    }
+    r.n_new = end - r.first;
+    if (r.length < 0 || (uint32_t)r.length > bt.max_length || (uint32_t)r.n_new > bt.max_new ||
+        ((uint64_t)bt.table_width << page_shift) < (uint64_t)r.length) {
+        atomicOr(status, kStatusGeometry);
+        r.length = 0;
+    }
+    return r;
+}
+
+// Page number of entry j of request b's row (j < table_width).  A number
+// outside the cache sets TC_STATUS_GEOMETRY and gives -1.
+__device__ __forceinline__ int32_t load_page(const BatchView &bt, uint32_t n_pages, uint32_t b, uint32_t j,
+                                             uint32_t *status) {
+    const int32_t p = bt.page_table[(uint64_t)b * bt.ld_table + j];
+    if (p < 0 || (uint32_t)p >= n_pages) {
+        atomicOr(status, kStatusGeometry);
+        return -1;
+    }
+    return p;
+}
+
+// Positions [lo, hi) that the new token at cache position p sees.
+__device__ __forceinline__ void visible(int32_t p, int32_t length, int causal, int32_t window, int32_t &lo,
+                                        int32_t &hi) {
+    lo = window > 0 ? max(p - window + 1, 0) : 0;
+    hi = causal ? min(p + 1, length) : window > 0 ? min(p + window, length) : length;
+}
+#endif
+
+// Host-side checks shared by the entry points; nullptr: fine.
+const char *check_cache(const tc_paged_cache *c, CacheView &v);
+const char *check_batch(const tc_paged_batch *b, BatchView &v);
+// Whether [a][b] rows of `width` elements at strides ld_a, ld_b share elements.
+bool rows_overlap(uint64_t a, uint64_t ld_a, uint64_t b, uint64_t ld_b, uint64_t width);
+
+}  // namespace tc

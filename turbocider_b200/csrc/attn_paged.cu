@@ -1,0 +1,556 @@
+// Attention of a step's new tokens over a paged cache
+// (tc_cuda_paged_attention): out = softmax(scale q K^T) V.
+//
+// The query heads that share a cache head are packed with the request's new
+// tokens into rows (row r: token r / group, head r % group), so K and V are
+// read once for all of them.  This file has the kernel for few rows (single
+// tokens, a few drafted ones): bytes bound, the floor is one read of K and V.
+//
+// A CTA takes up to 16 rows (one mma.sync tile; with so few rows the tensor
+// work is a small part of the memory time, so the padding costs nothing) of
+// one cache head and one chunk of the cache; its four warps take 16-key steps
+// in turn, each with its own running maximum, sum and output in registers, so
+// the loop has no CTA-wide synchronisation.  Each warp keeps a ring of TMA
+// boxes in flight (64 elements x up to 16 tokens of a page, 128-byte swizzle,
+// conflict-free for ldmatrix).  The warps' results are joined in shared
+// memory, the chunks' by the CTA that finishes last (partial outputs in the
+// workspace, added in chunk order, so the result does not depend on timing).
+//
+// Probabilities are rounded to the cache's 16-bit type for the P V product
+// (its relative error, 2^-9 or 2^-12 an element, averages out over the keys);
+// their sum is taken before the rounding.
+#include <cudaTypedefs.h>
+
+#include <cstring>
+#include <string>
+
+#include "attn.cuh"
+#include "attn_kernels.cuh"
+
+namespace tc {
+namespace {
+
+constexpr int kKeys = 16;        // keys of a warp's step
+constexpr int kWarps = 4;
+constexpr uint32_t kMaxChunk = 1024;
+
+template <int DP>
+struct FewLayout {
+    static constexpr int halves = DP / 64;
+    static constexpr uint32_t kv_bytes = kKeys * DP * 2;       // K of a step; V follows
+    static constexpr uint32_t stage = 2 * kv_bytes;
+    static constexpr int stages = DP == 64 ? 6 : 3;
+    static constexpr uint32_t ring = stages * stage;           // per warp
+    static constexpr uint32_t bar_off = kWarps * ring;
+    static constexpr uint32_t page_off = bar_off + kWarps * stages * 8;
+    static constexpr uint32_t ml_off = page_off + kMaxChunk / 8 * 4;    // [warp][16 rows][m, l]
+    static constexpr uint32_t misc_off = ml_off + kWarps * 16 * 8;
+    static constexpr uint32_t bytes = misc_off + 16 + 1024;
+    static_assert(kWarps * ring >= kWarps * 16 * DP * 4, "the join reuses the rings");
+};
+
+template <bool BF16>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if (BF16)
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+            "{%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+            "{%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <bool TRANS>
+__device__ __forceinline__ void ldsm4(uint32_t (&v)[4], uint32_t addr) {
+    if (TRANS)
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr) : "memory");
+    else
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr) : "memory");
+}
+
+// Two neighbouring 16-bit elements of q (pairs: 4-byte aligned) as one word.
+__device__ __forceinline__ uint32_t load_pair(const uint16_t *p, bool pairs, bool second) {
+    if (pairs) return *reinterpret_cast<const uint32_t *>(p);
+    return (uint32_t)p[0] | (second ? (uint32_t)p[1] << 16 : 0u);
+}
+
+template <int DP, bool BF16>
+__global__ void __launch_bounds__(kWarps * 32)
+    few_rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                    const __grid_constant__ AttnParams p) {
+    using L = FewLayout<DP>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t split = blockIdx.x, h = blockIdx.y, b = blockIdx.z / p.row_tiles, rt = blockIdx.z % p.row_tiles;
+    volatile uint32_t *abort_flag = reinterpret_cast<uint32_t *>(smem + L::misc_off);
+    uint32_t *last_flag = reinterpret_cast<uint32_t *>(smem + L::misc_off) + 1;
+
+    const Request rq = load_request(p.batch, p.page_shift, b, p.status);
+    const int32_t n_rows = rq.n_new * (int32_t)p.group, row0 = (int32_t)rt * 16;
+    if (row0 >= n_rows) return;
+    // keys that any row of the tile sees, and this CTA's share
+    const int32_t place0 = rq.length - rq.n_new;
+    const int32_t tok0 = row0 / (int32_t)p.group, tok1 = (min(row0 + 16, n_rows) - 1) / (int32_t)p.group;
+    int32_t lo, hi, unused;
+    visible(place0 + tok0, rq.length, p.causal, p.window, lo, unused);
+    visible(place0 + tok1, rq.length, p.causal, p.window, unused, hi);
+    const int32_t base = lo & ~(kKeys - 1);
+    const uint32_t n_split = hi > lo ? (uint32_t)(hi - base + (int32_t)p.chunk - 1) / p.chunk : 1u;
+    if (split >= n_split) return;
+    if (n_split > p.splits) {   // the launch was sized for a shorter span
+        if (threadIdx.x == 0) atomicOr(p.status, kStatusGeometry);
+        return;
+    }
+    const int32_t begin = base + (int32_t)(split * p.chunk), end = hi > lo ? min(hi, begin + (int32_t)p.chunk) : begin;
+
+    // ---- page numbers of the chunk, barriers
+    int32_t *pages = reinterpret_cast<int32_t *>(smem + L::page_off);
+    const uint32_t bars = su32(smem + L::bar_off) + warp * L::stages * 8;
+    if (end > begin) {
+        const uint32_t j0 = (uint32_t)begin >> p.page_shift, j1 = (uint32_t)(end - 1) >> p.page_shift;
+        for (uint32_t j = j0 + threadIdx.x; j <= j1; j += kWarps * 32)
+            pages[j - j0] = max(load_page(p.batch, p.n_pages, b, j, p.status), 0);
+    }
+    if (threadIdx.x == 0) *abort_flag = 0u;
+    if (lane == 0)
+        for (int i = 0; i < L::stages; ++i) bar_init(bars + 8 * i, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncthreads();
+
+    const uint32_t ring = su32(smem) + warp * L::ring;
+    const int32_t steps = (end - begin + kKeys - 1) / kKeys;
+    const uint32_t box = min((uint32_t)kKeys, 1u << p.page_shift);   // tokens of a TMA box
+    // Loads of the warp's step i (16 keys from `key`): boxes of both halves of
+    // each page piece that begins before the chunk's end.
+    auto issue = [&](int32_t i, uint32_t st) {
+        const int32_t key = begin + i * kKeys;
+        const uint32_t pieces = min((uint32_t)kKeys / box, (uint32_t)(end - key + (int32_t)box - 1) / box);
+        const uint32_t bar = bars + 8 * st, dst = ring + st * L::stage;
+        bar_expect_tx(bar, pieces * box * DP * 4);
+        for (uint32_t c = 0; c < pieces; ++c) {
+            const uint32_t pos = (uint32_t)key + c * box;
+            const int page = pages[(pos >> p.page_shift) - ((uint32_t)begin >> p.page_shift)];
+            const int token = (int)(pos & ((1u << p.page_shift) - 1));
+#pragma unroll
+            for (int hf = 0; hf < L::halves; ++hf) {
+                tma_load_4d(dst + hf * (kKeys * 128) + c * box * 128, &kmap, bar, hf * 64, token, (int)h, page);
+                tma_load_4d(dst + L::kv_bytes + hf * (kKeys * 128) + c * box * 128, &vmap, bar, hf * 64, token, (int)h,
+                            page);
+            }
+        }
+    };
+    if (lane == 0)
+        for (int32_t s = 0; s < L::stages; ++s)
+            if ((int32_t)warp + s * kWarps < steps) issue((int32_t)warp + s * kWarps, (uint32_t)s);
+    __syncwarp();
+
+    // ---- queries in registers (row-major A fragments)
+    const uint32_t g = lane / 4, t4 = lane % 4;
+    uint32_t qf[DP / 16][4];
+    int32_t row_lo[2], row_hi[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int32_t r = row0 + (int32_t)g + 8 * i;
+        const bool on = r < n_rows;
+        const int32_t tok = on ? r / (int32_t)p.group : 0;
+        visible(place0 + tok, rq.length, p.causal, p.window, row_lo[i], row_hi[i]);
+        if (!on) row_hi[i] = 0;
+        const uint16_t *q = p.q + (uint64_t)(rq.first + tok) * p.ld_q_token +
+                            (uint64_t)(h * p.group + (on ? r % (int32_t)p.group : 0)) * p.ld_q_head;
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const uint32_t d = ks * 16 + j * 8 + t4 * 2;
+                qf[ks][i + 2 * j] = on && d < p.head_dim ? load_pair(q + d, p.q_pairs, true) : 0u;
+            }
+    }
+
+    float o[DP / 8][4] = {};
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {};
+    uint32_t st = 0, ph = 0;
+    for (int32_t i = (int32_t)warp; i < steps; i += kWarps) {
+        const int32_t key = begin + i * kKeys;
+        const bool okw = bar_wait(bars + 8 * st, ph, abort_flag, p.status);
+        if (!__all_sync(0xffffffffu, okw)) break;
+        const uint32_t ks_addr = ring + st * L::stage, vs_addr = ks_addr + L::kv_bytes;
+        if (key < lo || key + kKeys > hi) {
+            // keys outside what the tile sees: their values must not reach the
+            // product even as 0 * NaN
+            for (uint32_t c = lane; c < kKeys * DP / 8; c += 32) {
+                const uint32_t r = c / (DP / 8), x = c % (DP / 8);
+                const int32_t j = key + (int32_t)r;
+                if (j < lo || j >= hi)
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};"
+                                 ::"r"(vs_addr + (x >> 3) * (kKeys * 128) + r * 128 + (((x & 7) ^ (r & 7)) << 4)), "r"(0)
+                                 : "memory");
+            }
+            fence_proxy_async();   // before a later copy into the stage
+            __syncwarp();
+        }
+        float s[2][4] = {};
+        const uint32_t lr = lane & 7, li = lane >> 3;
+        {
+            const uint32_t kr = (li >> 1) * 8 + lr;
+#pragma unroll
+            for (int ks = 0; ks < DP / 16; ++ks) {
+                const uint32_t x = ks * 2 + (li & 1);
+                uint32_t bf[4];
+                ldsm4<false>(bf, ks_addr + (x >> 3) * (kKeys * 128) + kr * 128 + (((x & 7) ^ lr) << 4));
+                mma16816<BF16>(s[0], qf[ks], bf[0], bf[1]);
+                mma16816<BF16>(s[1], qf[ks], bf[2], bf[3]);
+            }
+        }
+        // scale to powers of two, mask, running maximum
+        float mx[2] = {m[0], m[1]};
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int32_t j = key + n * 8 + (int32_t)t4 * 2 + (c & 1);
+                const bool seen = j >= row_lo[c >> 1] && j < row_hi[c >> 1];
+                s[n][c] = seen ? s[n][c] * p.scale_log2 : -INFINITY;
+                mx[c >> 1] = fmaxf(mx[c >> 1], s[n][c]);
+            }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+            mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+        }
+        if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
+            float al[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                al[r] = mx[r] > m[r] ? exp2f(m[r] - mx[r]) : 1.f;
+                l[r] *= al[r];
+                m[r] = mx[r];
+            }
+#pragma unroll
+            for (int n = 0; n < DP / 8; ++n) {
+                o[n][0] *= al[0];
+                o[n][1] *= al[0];
+                o[n][2] *= al[1];
+                o[n][3] *= al[1];
+            }
+        }
+        uint32_t pf[4];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const float mm = m[r] == -INFINITY ? 0.f : m[r];
+            float e[4];
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) e[n * 2 + c] = exp2f(s[n][r * 2 + c] - mm);
+            l[r] += (e[0] + e[1]) + (e[2] + e[3]);
+            pf[r] = pack16<BF16>(e[0], e[1]);
+            pf[r + 2] = pack16<BF16>(e[2], e[3]);
+        }
+        {
+            const uint32_t kr = (li & 1) * 8 + lr;
+#pragma unroll
+            for (int n = 0; n < DP / 16; ++n) {
+                const uint32_t x = n * 2 + (li >> 1);
+                uint32_t bf[4];
+                ldsm4<true>(bf, vs_addr + (x >> 3) * (kKeys * 128) + kr * 128 + (((x & 7) ^ lr) << 4));
+                mma16816<BF16>(o[2 * n], pf, bf[0], bf[1]);
+                mma16816<BF16>(o[2 * n + 1], pf, bf[2], bf[3]);
+            }
+        }
+        __syncwarp();   // every lane has read the stage
+        if (lane == 0 && i + L::stages * kWarps < steps) issue(i + L::stages * kWarps, st);
+        if (++st == L::stages) { st = 0; ph ^= 1; }
+    }
+    if (*abort_flag) {   // every copy issued has landed before the memory is reused or the CTA exits
+        for (int i = 0; i < L::stages; ++i) {
+            bar_wait(bars + 8 * i, 0, abort_flag, p.status, false);
+            bar_wait(bars + 8 * i, 1, abort_flag, p.status, false);
+        }
+    }
+
+    // ---- join the warps
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+    }
+    __syncthreads();   // the rings are free
+    float *ow = reinterpret_cast<float *>(smem) + warp * 16 * DP;
+    float2 *ml = reinterpret_cast<float2 *>(smem + L::ml_off);
+#pragma unroll
+    for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+            *reinterpret_cast<float2 *>(ow + (g + 8 * r) * DP + ((n * 8 + t4 * 2) ^ ((g & 3) * 8))) =
+                make_float2(o[n][2 * r], o[n][2 * r + 1]);
+    if (t4 == 0) {
+        ml[warp * 16 + g] = make_float2(m[0], l[0]);
+        ml[warp * 16 + g + 8] = make_float2(m[1], l[1]);
+    }
+    __syncthreads();
+    const uint32_t rows = (uint32_t)min(16, n_rows - row0);
+    const uint32_t tile = blockIdx.z * p.n_kv + h;
+    const float *oall = reinterpret_cast<const float *>(smem);
+    constexpr uint32_t quads = DP / 4;
+    // thread -> rows (threadIdx.x / quads) + ..., elements 4 * (threadIdx.x % quads)
+    for (uint32_t e = threadIdx.x; e < rows * quads; e += kWarps * 32) {
+        const uint32_t r = e / quads, d = (e % quads) * 4;
+        float mm = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, ml[w * 16 + r].x);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        float ll = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float2 v = ml[w * 16 + r];
+            const float a = v.x == -INFINITY ? 0.f : exp2f(v.x - mm);
+            const float4 x = *reinterpret_cast<const float4 *>(oall + (w * 16 + r) * DP + (d ^ ((r & 3) * 8)));
+            acc.x += a * x.x;
+            acc.y += a * x.y;
+            acc.z += a * x.z;
+            acc.w += a * x.w;
+            ll += a * v.y;
+        }
+        if (n_split == 1) {
+            store_row4<BF16>(p, rq, h, row0 + (int32_t)r, d, acc, mm, ll);
+        } else {
+            const uint64_t part = (uint64_t)tile * p.splits + split;
+            __stcg(reinterpret_cast<float4 *>(p.ws + p.ws_ml + (part * p.ws_rows + r) * DP + d), acc);
+            if (d == 0) __stcg(reinterpret_cast<float2 *>(p.ws) + part * p.ws_rows + r, make_float2(mm, ll));
+        }
+    }
+    if (n_split == 1) return;
+
+    // ---- the chunk that finishes last adds them all, in order
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const uint32_t before = atomicAdd(p.counters + tile, 1u);
+        *last_flag = before + 1 == n_split;
+        if (before + 1 == n_split) p.counters[tile] = 0u;
+    }
+    __syncthreads();
+    if (!*last_flag) return;
+    __threadfence();
+    for (uint32_t e = threadIdx.x; e < rows * quads; e += kWarps * 32) {
+        const uint32_t r = e / quads, d = (e % quads) * 4;
+        const float2 *mls = reinterpret_cast<const float2 *>(p.ws) + (uint64_t)tile * p.splits * p.ws_rows + r;
+        const float *os = p.ws + p.ws_ml + ((uint64_t)tile * p.splits * p.ws_rows + r) * DP + d;
+        float mm = -INFINITY, ll = 0.f;
+#pragma unroll 8
+        for (uint32_t s = 0; s < n_split; ++s) mm = fmaxf(mm, __ldcg(mls + (uint64_t)s * p.ws_rows).x);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+        for (uint32_t s = 0; s < n_split; ++s) {
+            const float2 v = __ldcg(mls + (uint64_t)s * p.ws_rows);
+            const float a = v.x == -INFINITY ? 0.f : exp2f(v.x - mm);
+            const float4 x = __ldcg(reinterpret_cast<const float4 *>(os + (uint64_t)s * p.ws_rows * DP));
+            acc.x += a * x.x;
+            acc.y += a * x.y;
+            acc.z += a * x.z;
+            acc.w += a * x.w;
+            ll += a * v.y;
+        }
+        store_row4<BF16>(p, rq, h, row0 + (int32_t)r, d, acc, mm, ll);
+    }
+}
+
+template <int DP, bool BF16>
+cudaError_t launch_few(const CUtensorMap &km, const CUtensorMap &vm, const AttnParams &p, dim3 grid, cudaStream_t s) {
+    using L = FewLayout<DP>;
+    auto kernel = few_rows_kernel<DP, BF16>;
+    static DeviceCache cache;
+    int unused = 0;
+    cudaError_t e = per_device(cache, unused, [&](int &) {
+        return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::bytes);
+    });
+    if (e != cudaSuccess) return e;
+    kernel<<<grid, kWarps * 32, L::bytes, s>>>(km, vm, p);
+    return cudaGetLastError();
+}
+
+template <int DP>
+cudaError_t launch_few_t(const CUtensorMap &km, const CUtensorMap &vm, const AttnParams &p, bool bf16, dim3 grid,
+                         cudaStream_t s) {
+    return bf16 ? launch_few<DP, true>(km, vm, p, grid, s) : launch_few<DP, false>(km, vm, p, grid, s);
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+    static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+        void *ptr = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+        return static_cast<PFN_cuTensorMapEncodeTiled_v12000>(nullptr);
+    }();
+    return fn;
+}
+
+// [page][head][token][d] of K or V as a map of 64-element x box_tokens boxes
+// with the 128-byte swizzle; elements past head_dim are filled with zeros.
+bool encode_cache(CUtensorMap *map, const uint16_t *base, const CacheView &c, uint32_t box_tokens, bool bf16) {
+    auto enc = encode_fn();
+    if (!enc) return false;
+    const cuuint64_t dims[4] = {c.head_dim, c.page_size, c.n_heads, c.n_pages};
+    // the stride of a dimension of one element is never used but must be valid
+    const uint64_t any = (uint64_t)c.head_dim * 2;
+    const cuuint64_t strides[3] = {c.ld_token * 2, c.n_heads > 1 ? c.ld_head * 2 : any, c.n_pages > 1 ? c.ld_page * 2 : any};
+    const cuuint32_t box[4] = {64u, box_tokens, 1u, 1u};
+    const cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
+    return enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+               const_cast<uint16_t *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int fail(const char *reason) {
+    set_last_error(reason);
+    return TC_CUDA_FAIL;
+}
+int ok() {
+    set_last_error("");
+    return TC_CUDA_OK;
+}
+int cuda_fail(const char *what, cudaError_t e) {
+    set_last_error(std::string(what) + ": " + cudaGetErrorString(e));
+    return TC_CUDA_FAIL;
+}
+
+// Grows the context's split workspace; the counters start at zero and every
+// complete kernel leaves them so.
+int ensure_split(tc_cuda_ctx *ctx, size_t floats, size_t counters, cudaStream_t s) {
+    if (floats > ctx->attn_ws_floats) {
+        if (ctx->attn_ws) cudaFree(ctx->attn_ws);
+        ctx->attn_ws = nullptr;
+        ctx->attn_ws_floats = 0;
+        const cudaError_t e = cudaMalloc(&ctx->attn_ws, floats * sizeof(float));
+        if (e != cudaSuccess) return cuda_fail("attention workspace allocation", e);
+        ctx->attn_ws_floats = floats;
+    }
+    if (counters > ctx->attn_counters_n) {
+        if (ctx->attn_counters) cudaFree(ctx->attn_counters);
+        ctx->attn_counters = nullptr;
+        ctx->attn_counters_n = 0;
+        cudaError_t e = cudaMalloc(&ctx->attn_counters, counters * sizeof(uint32_t));
+        if (e == cudaSuccess) e = cudaMemsetAsync(ctx->attn_counters, 0, counters * sizeof(uint32_t), s);
+        if (e != cudaSuccess) return cuda_fail("attention counter allocation", e);
+        ctx->attn_counters_n = counters;
+    }
+    return TC_CUDA_OK;
+}
+
+struct CurrentDevice {
+    int previous = -1;
+    explicit CurrentDevice(int device) {
+        if (cudaGetDevice(&previous) != cudaSuccess) previous = -1;
+        if (previous != device) cudaSetDevice(device);
+        else previous = -1;
+    }
+    ~CurrentDevice() {
+        if (previous >= 0) cudaSetDevice(previous);
+    }
+};
+
+int attend(tc_cuda_ctx *ctx, const tc_paged_cache *cache, const tc_paged_batch *batch, const tc_attention *a,
+           cudaStream_t s) {
+    CacheView c{};
+    AttnParams p{};
+    if (!ctx || !a) return fail("null argument");
+    if (const char *e = check_cache(cache, c)) return fail(e);
+    if (const char *e = check_batch(batch, p.batch)) return fail(e);
+    if (!a->n_heads || a->n_heads % c.n_heads) return fail("n_heads must be a multiple of the cache's heads");
+    if (!(a->scale == a->scale) || std::isinf(a->scale)) return fail("scale must be finite");
+    if (a->window < 0) return fail("window must not be negative");
+    if (!p.batch.n_tokens) return ok();
+    if (!a->q || !a->out) return fail("null argument");
+    if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->out)) % 2 ||
+        reinterpret_cast<uintptr_t>(a->lse) % 4)
+        return fail("misaligned pointer");
+    if ((a->ld_q_token | a->ld_q_head | a->ld_out_token | a->ld_out_head) >> 38)
+        return fail("invalid/overlapping head stride");
+    if (rows_overlap(p.batch.n_tokens, a->ld_out_token, a->n_heads, a->ld_out_head, c.head_dim))
+        return fail("invalid/overlapping head stride");
+    if (!p.batch.max_new) return fail("max_new must not be 0 where there are tokens");
+    const uint64_t group = a->n_heads / c.n_heads;
+    if (c.n_heads > 65535 || group * p.batch.max_new > 0x7fffffffu) return fail("too many heads");
+    p.q = static_cast<const uint16_t *>(a->q);
+    p.out = static_cast<uint16_t *>(a->out);
+    p.lse = a->lse;
+    p.ld_q_token = a->ld_q_token;
+    p.ld_q_head = a->ld_q_head;
+    p.ld_out_token = a->ld_out_token;
+    p.ld_out_head = a->ld_out_head;
+    p.n_kv = c.n_heads;
+    p.group = (uint32_t)group;
+    p.head_dim = c.head_dim;
+    p.page_shift = c.page_shift;
+    p.n_pages = c.n_pages;
+    p.causal = a->causal != 0;
+    p.window = a->window > kMaxLength ? kMaxLength : a->window;
+    p.scale_log2 = a->scale * 1.4426950408889634f;   // exp(x) = 2^(x log2 e)
+    p.status = ctx->status;
+    p.q_pairs = !(reinterpret_cast<uintptr_t>(a->q) % 4) && !(a->ld_q_token % 2) && !(a->ld_q_head % 2);
+    p.out_quads = !(reinterpret_cast<uintptr_t>(a->out) % 8) && !(a->ld_out_token % 4) && !(a->ld_out_head % 4);
+    const bool bf16 = cache->dtype == TC_DTYPE_BF16;
+
+    // longest span of keys one tile of rows sees
+    uint64_t span = p.batch.max_length;
+    if (p.window) {
+        const uint64_t reach = (uint64_t)p.window * (p.causal ? 1 : 2) + p.batch.max_new;
+        if (reach < span) span = reach;
+    }
+    span += kKeys;   // the first key is rounded down to a step
+    CurrentDevice guard(ctx->device);
+
+    p.row_tiles = (uint32_t)((group * p.batch.max_new + 15) / 16);
+    const uint64_t units = (uint64_t)p.batch.n_seq * p.row_tiles;
+    if (units > 65535) return fail("too many tokens or requests");
+    // Chunk of the cache per CTA: short enough that the largest possible work
+    // is about six CTAs for each one that fits on the GPU (two per SM), at
+    // least 128 keys, at most what the page list holds.
+    const uint64_t want = (uint64_t)ctx->sm_count * 2 * 6;
+    uint64_t chunk = (span * units * c.n_heads + want - 1) / want;
+    chunk = (chunk + 63) / 64 * 64;
+    if (chunk < 128) chunk = 128;
+    if (chunk > kMaxChunk) chunk = kMaxChunk;
+    p.chunk = (uint32_t)chunk;
+    p.splits = (uint32_t)((span + chunk - 1) / chunk);
+    p.ws_rows = (uint32_t)(group * p.batch.max_new < 16 ? group * p.batch.max_new : 16);
+    const uint32_t dp = c.head_dim <= 64 ? 64 : c.head_dim <= 128 ? 128 : 256;
+    if (p.splits > 1) {
+        const uint64_t parts = units * c.n_heads * p.splits * p.ws_rows;
+        p.ws_ml = (parts * 2 + 3) / 4 * 4;
+        if (ensure_split(ctx, p.ws_ml + parts * dp, units * c.n_heads, s)) return TC_CUDA_FAIL;
+        p.ws = ctx->attn_ws;
+        p.counters = ctx->attn_counters;
+    }
+    CUtensorMap km, vm;
+    const uint32_t box = c.page_size < kKeys ? c.page_size : kKeys;
+    if (!encode_cache(&km, c.k, c, box, bf16) || !encode_cache(&vm, c.v, c, box, bf16))
+        return fail("the cache cannot be described to TMA");
+    const dim3 grid(p.splits, c.n_heads, (uint32_t)units);
+    cudaError_t e = dp == 64 ? launch_few_t<64>(km, vm, p, bf16, grid, s)
+                  : dp == 128 ? launch_few_t<128>(km, vm, p, bf16, grid, s)
+                              : launch_few_t<256>(km, vm, p, bf16, grid, s);
+    return e == cudaSuccess ? ok() : cuda_fail("paged attention launch", e);
+}
+
+}  // namespace
+}  // namespace tc
+
+extern "C" int tc_cuda_paged_attention(tc_cuda_ctx *ctx, const tc_paged_cache *cache, const tc_paged_batch *batch,
+                                       const tc_attention *attention, void *stream) {
+    try {
+        return tc::attend(ctx, cache, batch, attention, static_cast<cudaStream_t>(stream));
+    } catch (...) {
+        return TC_CUDA_FAIL;
+    }
+}

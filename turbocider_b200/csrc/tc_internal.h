@@ -32,6 +32,12 @@ struct tc_cuda_ctx {
     cudaEvent_t push_fork = nullptr, push_join[8] = {};
     float *split_ws = nullptr;       // split-K partial products of the tensor-core GEMM
     size_t split_ws_floats = 0;
+    // Split attention: partial outputs with their softmax statistics, and one
+    // arrival counter per group of splits, kept at 0 (both grow on demand).
+    float *attn_ws = nullptr;
+    size_t attn_ws_floats = 0;
+    uint32_t *attn_counters = nullptr;
+    size_t attn_counters_n = 0;
     // Streaming GGUF loader (tc_cuda_weight_load_gguf): two pinned host and
     // two device staging slots (grow-only), its stream and per-slot events.
     void *load_host[2] = {}, *load_dev[2] = {};

@@ -87,6 +87,37 @@ class Epilogue(C.Structure):
                 ("ld_gate", _u64), ("seg_gate", C.POINTER(_i32)), ("residual", _vp), ("ld_residual", _u64)]
 
 
+class _Heads(C.Structure):
+    """struct tc_heads."""
+    _fields_ = [("x", _vp), ("out", _vp), ("weight", _vp), ("ld_token", _u64), ("ld_head", _u64),
+                ("ld_out_token", _u64), ("ld_out_head", _u64), ("n_heads", _u32), ("reserved", _u32)]
+
+
+class _Rope(C.Structure):
+    """struct tc_rope."""
+    _fields_ = [("freq", _vp), ("positions", _vp), ("rotary_dim", _u32), ("layout", _u32), ("n_axes", _u32),
+                ("sections", _u32 * 4), ("amplitude", C.c_float)]
+
+
+class _PagedCache(C.Structure):
+    """struct tc_paged_cache."""
+    _fields_ = [("k", _vp), ("v", _vp), ("ld_page", _u64), ("ld_head", _u64), ("ld_token", _u64), ("n_pages", _u32),
+                ("page_size", _u32), ("n_heads", _u32), ("head_dim", _u32), ("dtype", _u32), ("reserved", _u32)]
+
+
+class _PagedBatch(C.Structure):
+    """struct tc_paged_batch."""
+    _fields_ = [("new_offsets", _vp), ("lengths", _vp), ("page_table", _vp), ("n_seq", _u32), ("table_width", _u32),
+                ("ld_table", _u32), ("n_tokens", _u32), ("max_new", _u32), ("max_length", _u32)]
+
+
+class _Attention(C.Structure):
+    """struct tc_attention."""
+    _fields_ = [("q", _vp), ("out", _vp), ("lse", _vp), ("ld_q_token", _u64), ("ld_q_head", _u64),
+                ("ld_out_token", _u64), ("ld_out_head", _u64), ("n_heads", _u32), ("causal", _i32), ("window", _i32),
+                ("scale", C.c_float)]
+
+
 EXPORTS = {
     # name: (restype, argtypes)
     "tc_cuda_abi_version": (_u32, []),
@@ -144,6 +175,14 @@ EXPORTS = {
     "tc_cuda_weight_load_gguf": (C.c_int, [_vp, _vp, _u64, _u64, _u64, _u64, _vp, C.POINTER(_vp),
                                            C.POINTER(LoadStats)]),
     "tc_gguf_validate_split": (C.c_int, [C.POINTER(_vp), _u32]),
+    "tc_rope_freqs": (C.c_int, [_u32, C.c_double, _u32, C.c_double, C.c_double, C.c_double, C.c_double, _vp,
+                                C.POINTER(C.c_float)]),
+    "tc_cuda_qk_norm_rope": (C.c_int, [_vp, C.POINTER(_Heads), C.POINTER(_Heads), _u64, _u32, C.c_int, C.c_int,
+                                       C.c_float, C.POINTER(_Rope), _vp]),
+    "tc_cuda_kv_append": (C.c_int, [_vp, C.POINTER(_PagedCache), C.POINTER(_PagedBatch), C.POINTER(_Heads),
+                                    C.POINTER(_Heads), C.POINTER(_Heads), C.c_int, C.c_float, C.POINTER(_Rope), _vp]),
+    "tc_cuda_paged_attention": (C.c_int, [_vp, C.POINTER(_PagedCache), C.POINTER(_PagedBatch),
+                                          C.POINTER(_Attention), _vp]),
 }
 
 
@@ -502,6 +541,212 @@ def small_static_status(device: int = 0, clear: bool = True) -> int:
     bits = _u32()
     _check(lib().tc_cuda_small_static_status(device, C.byref(bits), int(clear)))
     return bits.value
+
+
+# ------------------------------------------------------------ attention
+_ROPE_LAYOUTS = {"half": 0, "interleaved": 1}
+_ROPE_SCALINGS = {"plain": 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4}
+_dtype_ids: dict = {}
+
+
+def _dtype_id(t) -> int:
+    if not _dtype_ids:
+        import torch
+        _dtype_ids.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+    if t.dtype not in _dtype_ids:
+        raise BackendError("tensors must be f32, f16 or bf16")
+    return _dtype_ids[t.dtype]
+
+
+def _ints(t, what: str, dims: int) -> int:
+    """Address of a contiguous int32 device tensor."""
+    if str(t.dtype) != "torch.int32" or not t.is_cuda or t.dim() != dims or not t.is_contiguous():
+        raise BackendError(f"{what} must be a contiguous int32 device tensor of {dims} dimension(s)")
+    return t.data_ptr()
+
+
+def rope_freqs(rotary_dim: int, theta: float = 10000.0, scaling: str = "plain", factor: float = 1.0,
+               trained_length: float = 0.0, beta_fast: float = 32.0, beta_slow: float = 1.0, device=None):
+    """(freq, amplitude) of a rotation for Rope: freq a float64 tensor
+    [rotary_dim / 2] of radians per position on `device` (None: the CPU).
+    scaling: "plain", "linear", "ntk", "yarn" or "bands" (struct tc_rope's
+    helper tc_rope_freqs has the formulas)."""
+    import torch
+    if scaling not in _ROPE_SCALINGS:
+        raise BackendError("unknown rotation scaling")
+    freq = torch.empty(max(rotary_dim // 2, 1), dtype=torch.float64)
+    amplitude = C.c_float()
+    _check(lib().tc_rope_freqs(rotary_dim, theta, _ROPE_SCALINGS[scaling], factor, trained_length, beta_fast,
+                               beta_slow, freq.data_ptr(), C.byref(amplitude)))
+    return (freq if device is None else freq.to(device)), amplitude.value
+
+
+class Rope:
+    """A position rotation (struct tc_rope).  freq: float64 device tensor of
+    radians per position, one for each rotated pair (rope_freqs).  positions:
+    int32 device tensor [tokens] or [tokens, axes]; None with kv_append: each
+    token's place in its cache.  layout: "half" (pairs i, i + rotary_dim / 2)
+    or "interleaved" (2i, 2i + 1).  sections: pairs of each axis."""
+
+    __slots__ = ("c", "freq", "positions")
+
+    def __init__(self, freq, positions=None, layout: str = "half", sections=None, amplitude: float = 1.0):
+        if str(freq.dtype) != "torch.float64" or not freq.is_cuda or freq.dim() != 1 or not freq.is_contiguous():
+            raise BackendError("freq must be a contiguous float64 device vector")
+        if layout not in _ROPE_LAYOUTS:
+            raise BackendError("invalid rotation layout")
+        axes = 1 if positions is None or positions.dim() == 1 else positions.shape[1]
+        sections = [freq.numel()] if sections is None else list(sections)
+        if axes != len(sections) or axes > 4:
+            raise BackendError("one section for each of 1 to 4 position axes")
+        self.freq, self.positions = freq, positions
+        c = self.c = _Rope()
+        c.freq = freq.data_ptr()
+        c.positions = None if positions is None else _ints(positions, "positions", positions.dim())
+        c.rotary_dim, c.layout, c.n_axes, c.amplitude = 2 * freq.numel(), _ROPE_LAYOUTS[layout], axes, amplitude
+        for i, n in enumerate(sections):
+            c.sections[i] = n
+
+
+class PagedCache:
+    """Keys and values in pages (struct tc_paged_cache): two f16 or bf16
+    device tensors [pages, heads, page_size, head_dim], or with
+    token_major=True [pages, page_size, heads, head_dim], of the same strides,
+    the last one contiguous."""
+
+    __slots__ = ("c", "k", "v", "dtype", "head_dim", "n_heads", "page_size")
+
+    def __init__(self, k, v, token_major: bool = False):
+        if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype:
+            raise BackendError("keys and values must be 4-dimensional tensors of the same shape, strides and type")
+        if not k.is_cuda or k.device != v.device or k.stride(3) != 1:
+            raise BackendError("the cache must be device tensors with a contiguous head dimension")
+        token, head = (1, 2) if token_major else (2, 1)
+        self.k, self.v, self.dtype = k, v, k.dtype
+        self.head_dim, self.n_heads, self.page_size = k.shape[3], k.shape[head], k.shape[token]
+        c = self.c = _PagedCache()
+        c.k, c.v, c.dtype = k.data_ptr(), v.data_ptr(), _dtype_id(k)
+        c.ld_page, c.ld_head, c.ld_token = k.stride(0), k.stride(head), k.stride(token)
+        c.n_pages, c.page_size, c.n_heads, c.head_dim = k.shape[0], self.page_size, self.n_heads, self.head_dim
+
+
+class PagedBatch:
+    """The new tokens of a step (struct tc_paged_batch): int32 device tensors
+    new_offsets [requests + 1], lengths [requests] (cached tokens, the new
+    ones included) and page_table [requests, width]; max_new and max_length
+    bound the new tokens and the length of every request."""
+
+    __slots__ = ("c", "tensors")
+
+    def __init__(self, new_offsets, lengths, page_table, max_new: int, max_length: int):
+        n = lengths.numel()
+        if new_offsets.numel() != n + 1 or page_table.dim() != 2 or page_table.shape[0] != n:
+            raise BackendError("new_offsets, lengths and page_table must have requests + 1, requests and requests rows")
+        if str(page_table.dtype) != "torch.int32" or not page_table.is_cuda or \
+                (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+            raise BackendError("page_table must be an int32 device tensor with contiguous rows")
+        if max_new < 0 or max_length < 0:
+            raise BackendError("max_new and max_length must not be negative")
+        self.tensors = (new_offsets, lengths, page_table)
+        c = self.c = _PagedBatch()
+        c.new_offsets, c.lengths = _ints(new_offsets, "new_offsets", 1), _ints(lengths, "lengths", 1)
+        c.page_table, c.n_seq, c.table_width = page_table.data_ptr(), n, page_table.shape[1]
+        c.ld_table = page_table.stride(0) if n > 1 else page_table.shape[1]
+        c.max_new, c.max_length = max_new, max_length
+
+
+def _heads(x, out, weight, what: str):
+    """struct tc_heads of a [tokens, heads, head_dim] device tensor."""
+    if x.dim() != 3 or not x.is_cuda or (x.stride(2) != 1 and x.shape[2] > 1):
+        raise BackendError(f"{what} must be a device tensor [tokens, heads, head_dim] with a contiguous last dimension")
+    h = _Heads()
+    h.x, h.n_heads = x.data_ptr(), x.shape[1]
+    h.ld_token, h.ld_head = x.stride(0), x.stride(1)
+    if out is not None:
+        if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or \
+                (out.stride(2) != 1 and out.shape[2] > 1):
+            raise BackendError(f"the result of {what} must have its shape, type and device")
+        h.out, h.ld_out_token, h.ld_out_head = out.data_ptr(), out.stride(0), out.stride(1)
+    if weight is not None:
+        if str(weight.dtype) != "torch.float32" or weight.shape != x.shape[2:] or not weight.is_contiguous() or \
+                weight.device != x.device:
+            raise BackendError("norm weights must be float32 device vectors of head_dim elements")
+        h.weight = weight.data_ptr()
+    return h
+
+
+def _fresh(x):
+    """A contiguous tensor of x's shape, type and device."""
+    return x.new_empty(x.shape)
+
+
+def qk_norm_rope(ctx: Context, q, k=None, rope: Rope | None = None, q_weight=None, k_weight=None,
+                 eps: float | None = None, q_out=None, k_out=None, stream=None):
+    """RMS norm over each head (eps None: no norm) and position rotation (rope
+    None: none) of query and key heads [tokens, heads, head_dim] in one
+    launch.  Weights: f32 [head_dim].  q_out / k_out may be q / k.  Returns
+    (q_out, k_out)."""
+    q_out = _fresh(q) if q_out is None else q_out
+    hq = _heads(q, q_out, q_weight, "q")
+    hk = None
+    if k is not None:
+        if k.dtype != q.dtype or k.device != q.device or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+            raise BackendError("q and k must share their type, device, tokens and head_dim")
+        k_out = _fresh(k) if k_out is None else k_out
+        hk = _heads(k, k_out, k_weight, "k")
+    if rope is not None and rope.positions is not None and rope.positions.shape[0] != q.shape[0]:
+        raise BackendError("one position for each token")
+    _check(lib().tc_cuda_qk_norm_rope(ctx.handle, hq, hk, q.shape[0], q.shape[2], _dtype_id(q), int(eps is not None),
+                                      eps or 0.0, None if rope is None else rope.c, _stream_ptr(stream)))
+    return q_out, k_out
+
+
+def kv_append(ctx: Context, cache: PagedCache, batch: PagedBatch, k, v, rope: Rope | None = None, q=None,
+              q_weight=None, k_weight=None, eps: float | None = None, q_out=None, stream=None):
+    """Writes the step's keys (normed with eps not None, rotated with rope)
+    and values [tokens, heads, head_dim] to the cache and, in the same launch,
+    norms and rotates the queries.  Returns q_out (None without q)."""
+    if k.dtype != cache.dtype or v.dtype != cache.dtype or k.shape != v.shape or k.shape[2] != cache.head_dim:
+        raise BackendError("keys and values must have the cache's type and head_dim")
+    if rope is not None and rope.positions is not None and rope.positions.shape[0] != k.shape[0]:
+        raise BackendError("one position for each token")
+    hq = None
+    if q is not None:
+        if q.dtype != cache.dtype or q.shape[0] != k.shape[0] or q.shape[2] != cache.head_dim:
+            raise BackendError("queries must have the cache's type and head_dim and one row for each key")
+        q_out = _fresh(q) if q_out is None else q_out
+        hq = _heads(q, q_out, q_weight, "q")
+    batch.c.n_tokens = k.shape[0]
+    _check(lib().tc_cuda_kv_append(ctx.handle, cache.c, batch.c, _heads(k, None, k_weight, "k"),
+                                   _heads(v, None, None, "v"), hq, int(eps is not None), eps or 0.0,
+                                   None if rope is None else rope.c, _stream_ptr(stream)))
+    return q_out if q is not None else None
+
+
+def paged_attention(ctx: Context, cache: PagedCache, batch: PagedBatch, q, scale: float | None = None,
+                    causal: bool = True, window: int = 0, out=None, return_lse: bool = False, stream=None):
+    """softmax(scale q K^T) V of the step's queries [tokens, heads, head_dim]
+    over each request's cache (scale None: head_dim ** -0.5); query heads share
+    cache heads in equal groups.  window > 0: only positions nearer than that.
+    Returns out, or (out, lse) with lse f32 [tokens, heads]."""
+    import torch
+    if q.dim() != 3 or q.dtype != cache.dtype or q.device != cache.k.device or q.shape[2] != cache.head_dim or \
+            q.stride(2) != 1:
+        raise BackendError("queries must be [tokens, heads, head_dim] of the cache's type, device and head_dim")
+    if out is None:
+        out = _fresh(q)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(2) != 1:
+        raise BackendError("the result must have the queries' shape, type and device")
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
+    a = _Attention()
+    a.q, a.out, a.lse = q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else None
+    a.ld_q_token, a.ld_q_head = q.stride(0), q.stride(1)
+    a.ld_out_token, a.ld_out_head = out.stride(0), out.stride(1)
+    a.n_heads, a.causal, a.window = q.shape[1], int(causal), window
+    a.scale = q.shape[2] ** -0.5 if scale is None else scale
+    batch.c.n_tokens = q.shape[0]
+    _check(lib().tc_cuda_paged_attention(ctx.handle, cache.c, batch.c, a, _stream_ptr(stream)))
+    return (out, lse) if return_lse else out
 
 
 class GGUFError(BackendError):
