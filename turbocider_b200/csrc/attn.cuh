@@ -68,6 +68,22 @@ __device__ __forceinline__ int32_t load_page(const BatchView &bt, uint32_t n_pag
     return p;
 }
 
+// How many of the requests 1 .. n satisfy `before` (true for a prefix of
+// them), found by the warp 32 at a time.
+template <class F>
+__device__ __forceinline__ uint32_t count_prefix(uint32_t n, F &&before) {
+    const uint32_t lane = threadIdx.x & 31;
+    uint32_t lo = 0;   // the answer is in [lo, lo + n]
+    while (n > 0) {
+        const uint32_t step = (n + 31) / 32, i = (lane + 1) * step;
+        const bool yes = before(lo + min(i, n)) && i <= n;
+        const uint32_t c = __popc(__ballot_sync(0xffffffffu, yes));
+        lo += c * step;
+        n = min(n - c * step, step - 1);
+    }
+    return lo;
+}
+
 // Positions [lo, hi) that the new token at cache position p sees.
 __device__ __forceinline__ void visible(int32_t p, int32_t length, int causal, int32_t window, int32_t &lo,
                                         int32_t &hi) {

@@ -94,20 +94,10 @@ __device__ __forceinline__ void store_chunk(T *p, const Chunk<T> &c) {
     for (int i = 0; i < 4; ++i) p[i] = c.v[i];
 }
 
-// Request of token t: the number of requests whose end is <= t, found by the
-// warp 32 ends at a time (n_seq: t belongs to none).
+// Request of token t: the number of requests that end at or before it
+// (n_seq: t belongs to none).
 __device__ __forceinline__ uint32_t request_of(const BatchView &bt, int32_t t) {
-    const uint32_t lane = threadIdx.x & 31;
-    uint32_t lo = 0, n = bt.n_seq;   // the answer is in [lo, lo + n]
-    while (n > 0) {
-        const uint32_t step = (n + 31) / 32;
-        const uint32_t i = lo + min((lane + 1) * step, n);   // ends new_offsets[lo + 1 .. lo + n]
-        const bool le = bt.new_offsets[i] <= t;
-        const uint32_t c = __popc(__ballot_sync(0xffffffffu, le && (lane + 1) * step <= n));
-        lo += c * step;
-        n = min(n - c * step, step - 1);
-    }
-    return lo;
+    return count_prefix(bt.n_seq, [&](uint32_t b) { return bt.new_offsets[b] <= t; });
 }
 
 template <class T, bool HALF, bool APPEND, bool VEC>

@@ -25,7 +25,16 @@ struct AttnParams {
     float *ws;
     uint32_t *counters;
     bool q_pairs, out_quads;     // 4-byte loads of q / 8-byte stores of out are aligned
+    bool q_wide, out_wide;       // 16-byte loads of q / stores of out are aligned
+    uint32_t n_blocks;           // many rows: upper bound of the blocks of rows
+    bool negate_q;               // many rows: scale_log2 is positive, the sign goes to q
 };
+
+// Chunks of many rows (attn_chunk_sm100.cu), head_dim at most 128.
+constexpr int kChunkRows = 256;      // rows of a CTA: two tensor-core tiles
+constexpr int kChunkKeys = 128;      // keys of a step
+cudaError_t launch_chunk(const CUtensorMap &km, const CUtensorMap &vm, const AttnParams &p, bool bf16,
+                         cudaStream_t s);
 
 namespace {
 

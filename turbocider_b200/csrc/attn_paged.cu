@@ -21,7 +21,8 @@
 // their sum is taken before the rounding.
 #include <cudaTypedefs.h>
 
-#include <cstring>
+#include <algorithm>
+#include <cmath>
 #include <string>
 
 #include "attn.cuh"
@@ -33,6 +34,7 @@ namespace {
 constexpr int kKeys = 16;        // keys of a warp's step
 constexpr int kWarps = 4;
 constexpr uint32_t kMaxChunk = 1024;
+constexpr uint64_t kFewRows = 16;   // rows of a request up to which this file's kernel is used
 
 template <int DP>
 struct FewLayout {
@@ -507,12 +509,55 @@ int attend(tc_cuda_ctx *ctx, const tc_paged_cache *cache, const tc_paged_batch *
         const uint64_t reach = (uint64_t)p.window * (p.causal ? 1 : 2) + p.batch.max_new;
         if (reach < span) span = reach;
     }
-    span += kKeys;   // the first key is rounded down to a step
     CurrentDevice guard(ctx->device);
 
-    p.row_tiles = (uint32_t)((group * p.batch.max_new + 15) / 16);
+    const uint64_t rows_most = group * p.batch.max_new;
+    if (rows_most > kFewRows && c.head_dim <= 128) {
+        const uint64_t rows = (uint64_t)p.batch.n_tokens * group;
+        p.n_blocks = (uint32_t)(rows / kChunkRows + p.batch.n_seq);
+        p.q_wide = !(reinterpret_cast<uintptr_t>(a->q) % 16) && !(a->ld_q_token % 8) && !(a->ld_q_head % 8);
+        p.out_wide = !(reinterpret_cast<uintptr_t>(a->out) % 16) && !(a->ld_out_token % 8) && !(a->ld_out_head % 8);
+        p.negate_q = p.scale_log2 < 0.f;
+        p.scale_log2 = std::fabs(p.scale_log2);
+        if (p.scale_log2 < 1e-30f) p.scale_log2 = 1e-30f;   // 0 * -inf would lose the mask
+        // Shares of the keys: as many CTAs as make the busiest SM's work least,
+        // in steps of 128 keys plus kCtaSteps for what a CTA does besides, one
+        // CTA per SM, no share under kLeastSteps.
+        constexpr uint64_t kCtaSteps = 3, kLeastSteps = 3;
+        const uint64_t steps = (span + kChunkKeys - 1) / kChunkKeys + 1;
+        const uint64_t blocks = std::max<uint64_t>((rows + kChunkRows - 1) / kChunkRows, p.batch.n_seq);
+        uint64_t best = ~0ull, share = steps;
+        for (uint64_t n = 1; n <= 64 && (n == 1 || steps / n >= kLeastSteps); ++n) {
+            const uint64_t each = (steps + n - 1) / n, real = (steps + each - 1) / each;
+            const uint64_t waves = (blocks * c.n_heads * real + ctx->sm_count - 1) / ctx->sm_count;
+            const uint64_t cost = waves * (each + kCtaSteps + (real > 1 ? 1 : 0));
+            if (cost < best) {
+                best = cost;
+                share = each;
+            }
+        }
+        p.chunk = (uint32_t)(share * kChunkKeys);
+        p.splits = (uint32_t)((steps + share - 1) / share);
+        if ((uint64_t)p.n_blocks * c.n_heads * p.splits > 0x7fffffffu) return fail("too many tokens or requests");
+        const uint64_t dp = c.head_dim <= 64 ? 64 : 128;
+        if (p.splits > 1) {
+            const uint64_t parts = (uint64_t)p.n_blocks * c.n_heads * p.splits * kChunkRows;
+            p.ws_ml = parts * 2;
+            if (ensure_split(ctx, p.ws_ml + parts * dp, (size_t)p.n_blocks * c.n_heads, s)) return TC_CUDA_FAIL;
+            p.ws = ctx->attn_ws;
+            p.counters = ctx->attn_counters;
+        }
+        CUtensorMap km, vm;
+        const uint32_t box = c.page_size < kChunkKeys ? c.page_size : kChunkKeys;
+        if (!encode_cache(&km, c.k, c, box, bf16) || !encode_cache(&vm, c.v, c, box, bf16))
+            return fail("the cache cannot be described to TMA");
+        const cudaError_t e = launch_chunk(km, vm, p, bf16, s);
+        return e == cudaSuccess ? ok() : cuda_fail("paged attention launch", e);
+    }
+    p.row_tiles = (uint32_t)((rows_most + 15) / 16);
     const uint64_t units = (uint64_t)p.batch.n_seq * p.row_tiles;
     if (units > 65535) return fail("too many tokens or requests");
+    span += kKeys;   // the first key is rounded down to a step
     // Chunk of the cache per CTA: short enough that the largest possible work
     // is about six CTAs for each one that fits on the GPU (two per SM), at
     // least 128 keys, at most what the page list holds.
