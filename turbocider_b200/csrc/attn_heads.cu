@@ -7,13 +7,13 @@
 //
 // Bytes bound: every element is read once and written once (2 + 2 bytes for
 // 16-bit types) against about 10 flops.  A head is spread over the smallest
-// power-of-two group of lanes that gives each lane one unit of 8 elements: 4
-// pairs with both members in the same lane (two 4-element chunks half a
-// rotary width apart for the half layout, 8 neighbours for the interleaved
-// one), so the rotation needs no exchange and the norm one butterfly over the
-// group.  A block takes one token; a thread keeps its unit for all heads it
-// visits, so the angles, sines and cosines are formed once per thread and
-// serve every head.
+// power-of-two group of lanes that gives each lane one unit of 16 elements (8
+// for f32 and for odd sizes): two chunks half a rotary width apart for the
+// half layout, half a head apart for the interleaved one (whole sectors per
+// access), so that both members of every pair are in one lane, the rotation needs no exchange and the norm one
+// butterfly over the group.  A warp takes one token and some or all of its
+// heads, kBatch for each lane group at a time; the token's sines and cosines are
+// formed once per warp.
 //
 // The angle: freq / 2 pi is held as a 64-bit binary fraction of a turn and
 // multiplied by the position modulo 2^64, i.e. modulo one turn and exactly,
@@ -25,6 +25,7 @@
 #include <string>
 
 #include "attn.cuh"
+#include "kq_sm100.cuh"
 
 namespace tc {
 namespace {
@@ -39,13 +40,13 @@ struct HeadsView {
 
 struct HeadsParams {
     HeadsView q, k, v;           // v: copied to the cache (append only)
-    uint32_t head_dim, n_tokens, heads_per_block;
+    uint32_t head_dim, n_tokens, groups, heads_per_group;
     int rms_norm;
     float eps, inv_dim;
     // rotation
     const double *freq;
     const int32_t *positions;
-    uint32_t rotary_units, half, n_axes, axis_end[4];
+    uint32_t half, n_axes, axis_end[4];
     float amplitude;
     // append
     BatchView batch;
@@ -53,8 +54,7 @@ struct HeadsParams {
     uint32_t *status;
 };
 
-// Four elements in and out of fp32.
-__device__ __forceinline__ void unpack4(float4 v, float *f) { f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w; }
+// Elements in and out of fp32.
 template <class T>
 __device__ __forceinline__ float to_float(T v);
 template <>
@@ -72,26 +72,32 @@ __device__ __forceinline__ __half from_float<__half>(float v) { return __float2h
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-template <class T>
-struct alignas(4 * sizeof(T)) Chunk { T v[4]; };
+// A lane's unit of a head: two chunks of CH elements.
+template <class T, int CH>
+struct alignas(CH * sizeof(T) < 16 ? CH * sizeof(T) : 16) Chunk { T v[CH]; };
+template <class T, int CH>
+struct Unit { Chunk<T, CH> c[2]; };
 
-// VEC: 4-element chunks may be moved as one access.
-template <class T, bool VEC>
-__device__ __forceinline__ Chunk<T> load_chunk(const T *p) {
-    if (VEC) return *reinterpret_cast<const Chunk<T> *>(p);
-    Chunk<T> c;
+// WIDE: accesses of whole chunks are aligned.
+template <class T, int CH, bool WIDE>
+__device__ __forceinline__ void load_unit(Unit<T, CH> &u, const T *p, const uint32_t (&at)[2]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) c.v[i] = p[i];
-    return c;
-}
-template <class T, bool VEC>
-__device__ __forceinline__ void store_chunk(T *p, const Chunk<T> &c) {
-    if (VEC) {
-        *reinterpret_cast<Chunk<T> *>(p) = c;
-        return;
+    for (int k = 0; k < 2; ++k) {
+        if (WIDE) u.c[k] = *reinterpret_cast<const Chunk<T, CH> *>(p + at[k]);
+        else
+#pragma unroll
+            for (int i = 0; i < CH; ++i) u.c[k].v[i] = p[at[k] + i];
     }
+}
+template <class T, int CH, bool WIDE>
+__device__ __forceinline__ void store_unit(T *p, const uint32_t (&at)[2], const Unit<T, CH> &u) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) p[i] = c.v[i];
+    for (int k = 0; k < 2; ++k) {
+        if (WIDE) *reinterpret_cast<Chunk<T, CH> *>(p + at[k]) = u.c[k];
+        else
+#pragma unroll
+            for (int i = 0; i < CH; ++i) p[at[k] + i] = u.c[k].v[i];
+    }
 }
 
 // Request of token t: the number of requests that end at or before it
@@ -100,18 +106,147 @@ __device__ __forceinline__ uint32_t request_of(const BatchView &bt, int32_t t) {
     return count_prefix(bt.n_seq, [&](uint32_t b) { return bt.new_offsets[b] <= t; });
 }
 
-template <class T, bool HALF, bool APPEND, bool VEC>
-__global__ void __launch_bounds__(128) heads_kernel(const __grid_constant__ HeadsParams p) {
-    const uint32_t units = p.head_dim / 8;
-    const uint32_t lanes = units <= 1 ? 1u : 1u << (32 - __clz(units - 1));   // lanes per head
-    const uint32_t unit = threadIdx.x & (lanes - 1), slot = threadIdx.x / lanes, slots = blockDim.x / lanes;
-    const bool active = unit < units, rotates = unit < p.rotary_units;
-    // the unit's two chunks of four elements
-    const uint32_t c0 = rotates && HALF ? 4 * unit : 8 * unit;
-    const uint32_t c1 = rotates && HALF ? p.half + 4 * unit : 8 * unit + 4;
-    const uint32_t n_rot = p.q.n_heads + p.k.n_heads, n_all = n_rot + p.v.n_heads;
-    const uint32_t h_end = min((blockIdx.y + 1) * p.heads_per_block, n_all);
-    const uint64_t t = blockIdx.x;
+constexpr int kBlocks = 6;   // resident per SM (at most 80 registers a thread)
+constexpr int kWarps = 4, kBatch = 2;   // warps of a block; heads that a lane has in flight
+
+// What a lane keeps for every head it visits.
+struct Lane {
+    uint32_t at[2], lanes, slot, slots;   // elements where its chunks begin
+    bool active, rotates[2];              // chunk k is rotated
+    uint32_t pair[2];                     // pair of chunk k's first element
+};
+
+// Members of a unit's pairs as fp32: a[i], b[i] are elements i of its chunks
+// (half layout) or neighbours (the first half of them in chunk 0).
+template <class T, int CH, bool HALF>
+__device__ __forceinline__ void unpack(const Unit<T, CH> &u, float (&a)[CH], float (&b)[CH]) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+        a[i] = to_float<T>(HALF ? u.c[0].v[i] : u.c[2 * i / CH].v[2 * i % CH]);
+        b[i] = to_float<T>(HALF ? u.c[1].v[i] : u.c[2 * i / CH].v[2 * i % CH + 1]);
+    }
+}
+template <class T, int CH, bool HALF>
+__device__ __forceinline__ void pack(Unit<T, CH> &u, const float (&a)[CH], const float (&b)[CH]) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+        (HALF ? u.c[0].v[i] : u.c[2 * i / CH].v[2 * i % CH]) = from_float<T>(a[i]);
+        (HALF ? u.c[1].v[i] : u.c[2 * i / CH].v[2 * i % CH + 1]) = from_float<T>(b[i]);
+    }
+}
+// Two fp32 lanes in one operation (sm_100a).
+__device__ __forceinline__ uint64_t two(float lo, float hi) {
+    return f2pack(__float_as_uint(lo), __float_as_uint(hi));
+}
+
+// Heads [begin, end) of one kind, `slots` at a time: norm, rotation, store.
+// The heads of a batch are all read before the first is written (out may be x).
+template <class T, int CH, bool HALF, bool WIDE>
+__device__ __forceinline__ void turn_heads(const HeadsParams &p, const Lane &ln, const float2 *turn, const T *x, uint64_t ld_x, T *out,
+                                           uint64_t ld_out, const float *weight, uint32_t begin, uint32_t end,
+                                           bool store) {
+    if (begin >= end) return;
+    // a' = r (a wa cos - b wb sin), b' = r (b wb cos + a wa sin); a chunk past
+    // the rotated part keeps a' = r a wa, b' = r b wb
+    uint64_t aa[CH / 2], ab[CH / 2], bb[CH / 2], ba[CH / 2];
+#pragma unroll
+    for (int i = 0; i < CH; i += 2) {
+        float wa[2] = {1.f, 1.f}, wb[2] = {1.f, 1.f};
+        float2 cs[2] = {{1.f, 0.f}, {1.f, 0.f}};
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int e = i + k, c = HALF ? 0 : 2 * e / CH;   // chunk of a
+            if (weight) {
+                wa[k] = weight[HALF ? ln.at[0] + e : ln.at[c] + 2 * e % CH];
+                wb[k] = weight[HALF ? ln.at[1] + e : ln.at[c] + 2 * e % CH + 1];
+            }
+            if (ln.rotates[c]) cs[k] = turn[ln.pair[c] + (HALF ? e : e % (CH / 2))];
+        }
+        aa[i / 2] = two(wa[0] * cs[0].x, wa[1] * cs[1].x);
+        ab[i / 2] = two(-wb[0] * cs[0].y, -wb[1] * cs[1].y);
+        bb[i / 2] = two(wb[0] * cs[0].x, wb[1] * cs[1].x);
+        ba[i / 2] = two(wa[0] * cs[0].y, wa[1] * cs[1].y);
+    }
+    store = store && ln.active;
+    // (every lane runs every round: the butterfly of the norm needs them all)
+    for (uint32_t h0 = begin + ln.slot; h0 < end + ln.slot; h0 += kBatch * ln.slots) {
+        Unit<T, CH> u[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k)
+            load_unit<T, CH, WIDE>(u[k], x + min(h0 + k * ln.slots, end - 1) * ld_x, ln.at);
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            const uint32_t h = h0 + k * ln.slots;
+            float fa[CH], fb[CH];
+            unpack<T, CH, HALF>(u[k], fa, fb);
+            uint64_t a[CH / 2], b[CH / 2];
+#pragma unroll
+            for (int i = 0; i < CH; i += 2) {
+                a[i / 2] = two(fa[i], fa[i + 1]);
+                b[i / 2] = two(fb[i], fb[i + 1]);
+            }
+            float r = 1.f;
+            if (p.rms_norm) {
+                uint64_t s = f2mul(a[0], a[0]);
+#pragma unroll
+                for (int i = 1; i < CH / 2; ++i) s = f2fma(a[i], a[i], s);
+#pragma unroll
+                for (int i = 0; i < CH / 2; ++i) s = f2fma(b[i], b[i], s);
+                float s0, s1;
+                f2unpack(s, s0, s1);
+                float ss = ln.active ? s0 + s1 : 0.f;
+                for (uint32_t d = ln.lanes / 2; d > 0; d /= 2) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+                r = rsqrtf(ss * p.inv_dim + p.eps);
+            }
+            const uint64_t r2 = f2splat(r);
+#pragma unroll
+            for (int i = 0; i < CH / 2; ++i) {
+                uint64_t ya = f2mul(a[i], aa[i]), yb = f2mul(b[i], bb[i]);
+                if (ln.rotates[HALF ? 0 : 4 * i / CH]) {
+                    ya = f2fma(b[i], ab[i], ya);
+                    yb = f2fma(a[i], ba[i], yb);
+                }
+                f2unpack(f2mul(ya, r2), fa[2 * i], fa[2 * i + 1]);
+                f2unpack(f2mul(yb, r2), fb[2 * i], fb[2 * i + 1]);
+            }
+            if (store && h < end) {
+                pack<T, CH, HALF>(u[k], fa, fb);
+                store_unit<T, CH, WIDE>(out + h * ld_out, ln.at, u[k]);
+            }
+        }
+    }
+}
+
+template <class T, int CH, bool HALF, bool APPEND, bool WIDE>
+__global__ void __launch_bounds__(kWarps * 32, kBlocks) heads_kernel(const __grid_constant__ HeadsParams p) {
+    __shared__ float2 turns[kWarps][128];   // cos and sin of the token's pairs
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint64_t task = (uint64_t)blockIdx.x * kWarps + warp;
+    const uint64_t t = task / p.groups;
+    if (t >= p.n_tokens) return;
+    const uint32_t units = p.head_dim / (2 * CH);
+    Lane ln;
+    ln.lanes = units <= 1 ? 1u : 1u << (32 - __clz(units - 1));   // lanes per head
+    ln.slot = lane / ln.lanes;
+    ln.slots = 32 / ln.lanes;
+    const uint32_t own = lane & (ln.lanes - 1);
+    ln.active = own < units;
+    // (a lane without a unit reads the first one's and adds and stores nothing)
+    const uint32_t unit = ln.active ? own : 0u;
+    if (HALF) {
+        const uint32_t turned = p.half / CH;   // units that are rotated
+        ln.rotates[0] = ln.rotates[1] = unit < turned;
+        ln.at[0] = unit < turned ? CH * unit : 2 * p.half + CH * (unit - turned);
+        ln.at[1] = ln.at[0] + (unit < turned ? p.half : p.head_dim / 2 - p.half);
+        ln.pair[0] = ln.pair[1] = CH * unit;
+    } else {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            ln.at[k] = CH * unit + k * (p.head_dim / 2);
+            ln.rotates[k] = ln.at[k] < 2 * p.half;
+            ln.pair[k] = ln.at[k] / 2;
+        }
+    }
 
     int32_t position = 0;
     uint64_t k_base = 0;          // of head 0 in the cache
@@ -130,133 +265,83 @@ __global__ void __launch_bounds__(128) heads_kernel(const __grid_constant__ Head
         }
         position = max(at, 0);
     }
-
-    float cs[4], sn[4];
-    if (rotates) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t pair = 4 * unit + i;
-            int32_t pos = position;
-            if (p.positions) {
-                uint32_t axis = 0;
-                while (axis + 1 < p.n_axes && pair >= p.axis_end[axis]) ++axis;
-                pos = p.positions[t * p.n_axes + axis];
-            }
-            // freq in turns as a fraction of 2^64; negative frequencies wrap
-            // (two's complement), whole turns fall away
-            const double turns = p.freq[pair] * 0.15915494309189533577;   // 1 / (2 pi)
-            const uint64_t step = (uint64_t)__double2ull_rn((turns - floor(turns)) * 18446744073709551616.0);
-            const uint64_t phase = step * (uint64_t)(int64_t)pos;
-            sincospif((float)(int32_t)(phase >> 32) * 4.656612873077392578125e-10f, &sn[i], &cs[i]);   // 2^-31
-            sn[i] *= p.amplitude;
-            cs[i] *= p.amplitude;
+    for (uint32_t pair = lane; pair < p.half; pair += 32) {
+        int32_t pos = position;
+        if (p.positions) {
+            uint32_t axis = 0;
+            while (axis + 1 < p.n_axes && pair >= p.axis_end[axis]) ++axis;
+            pos = p.positions[t * p.n_axes + axis];
         }
+        // freq in turns as a fraction of 2^64 (negative ones wrap, whole turns
+        // fall away), times the position modulo 2^64
+        const double turn = p.freq[pair] * 0.15915494309189533577;   // 1 / (2 pi)
+        const uint64_t step = (uint64_t)__double2ull_rn((turn - floor(turn)) * 18446744073709551616.0);
+        const uint64_t phase = step * (uint64_t)(int64_t)pos;
+        float s, c;
+        sincospif((float)(int32_t)(phase >> 32) * 4.656612873077392578125e-10f, &s, &c);   // 2^-31
+        turns[warp][pair] = make_float2(c * p.amplitude, s * p.amplitude);
     }
+    __syncwarp();
 
-    // heads 0 .. : the queries', then the keys', then the values'
-#pragma unroll 4
-    for (uint32_t h = blockIdx.y * p.heads_per_block + slot; h < h_end + slot; h += slots) {
-        // (every lane runs the loop so that the butterfly below is complete)
-        const bool on = active && h < h_end;
-        const bool is_q = h < p.q.n_heads, is_v = h >= n_rot;
-        const HeadsView &hv = is_q ? p.q : is_v ? p.v : p.k;
-        const uint32_t hh = is_q ? h : is_v ? h - n_rot : h - p.q.n_heads;
-        const T *x = static_cast<const T *>(hv.x) + t * hv.ld_token + hh * hv.ld_head;
-        Chunk<T> a, b;
-        if (on) {
-            a = load_chunk<T, VEC>(x + c0);
-            b = load_chunk<T, VEC>(x + c1);
-        }
-        T *out;
-        if (APPEND && !is_q)
-            out = reinterpret_cast<T *>(is_v ? p.cache.v : p.cache.k) + k_base + hh * p.cache.ld_head;
-        else
-            out = static_cast<T *>(hv.out) + t * hv.ld_out_token + hh * hv.ld_out_head;
-        const bool store = on && (!APPEND || is_q || store_kv);
-        float fa[4], fb[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            fa[i] = on ? to_float<T>(a.v[i]) : 0.f;
-            fb[i] = on ? to_float<T>(b.v[i]) : 0.f;
-        }
-        if (p.rms_norm) {
-            float ss = 0.f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) ss += fa[i] * fa[i] + fb[i] * fb[i];
-            for (uint32_t d = lanes / 2; d > 0; d /= 2) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-            if (!is_v) {
-                const float r = rsqrtf(ss * p.inv_dim + p.eps);
-                float wa[4] = {1.f, 1.f, 1.f, 1.f}, wb[4] = {1.f, 1.f, 1.f, 1.f};
-                if (hv.weight && on) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        wa[i] = hv.weight[c0 + i];
-                        wb[i] = hv.weight[c1 + i];
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    fa[i] *= r * wa[i];
-                    fb[i] *= r * wb[i];
-                }
-            }
-        }
-        if (rotates && !is_v) {
-            if (HALF) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float u = fa[i], w = fb[i];
-                    fa[i] = u * cs[i] - w * sn[i];
-                    fb[i] = w * cs[i] + u * sn[i];
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float *e = i < 2 ? fa + 2 * i : fb + 2 * i - 4;
-                    const float u = e[0], w = e[1];
-                    e[0] = u * cs[i] - w * sn[i];
-                    e[1] = w * cs[i] + u * sn[i];
-                }
-            }
-        }
-        if (store) {
-            if (!is_v) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    a.v[i] = from_float<T>(fa[i]);
-                    b.v[i] = from_float<T>(fb[i]);
-                }
-            }
-            store_chunk<T, VEC>(out + c0, a);
-            store_chunk<T, VEC>(out + c1, b);
+    // this warp's share of the heads: the queries' come first, then the keys', then the values'
+    const uint32_t nq = p.q.n_heads, nk = p.k.n_heads, nv = p.v.n_heads;
+    const uint32_t h0 = (uint32_t)(task % p.groups) * p.heads_per_group, h1 = h0 + p.heads_per_group;
+    turn_heads<T, CH, HALF, WIDE>(p, ln, turns[warp], static_cast<const T *>(p.q.x) + t * p.q.ld_token, p.q.ld_head,
+                                  static_cast<T *>(p.q.out) + t * p.q.ld_out_token, p.q.ld_out_head, p.q.weight,
+                                  min(h0, nq), min(h1, nq), true);
+    const uint32_t k0 = min(max(h0, nq) - nq, nk), k1 = min(max(h1, nq) - nq, nk);
+    turn_heads<T, CH, HALF, WIDE>(p, ln, turns[warp], static_cast<const T *>(p.k.x) + t * p.k.ld_token, p.k.ld_head,
+                                  APPEND ? reinterpret_cast<T *>(p.cache.k) + k_base
+                                         : static_cast<T *>(p.k.out) + t * p.k.ld_out_token,
+                                  APPEND ? p.cache.ld_head : p.k.ld_out_head, p.k.weight, k0, k1,
+                                  !APPEND || store_kv);
+    if (APPEND && store_kv && ln.active) {   // values as they are
+        const uint32_t first = nq + nk, v0 = min(max(h0, first) - first, nv), v1 = min(max(h1, first) - first, nv);
+        const T *x = static_cast<const T *>(p.v.x) + t * p.v.ld_token;
+        T *out = reinterpret_cast<T *>(p.cache.v) + k_base;
+#pragma unroll 2
+        for (uint32_t h = v0 + ln.slot; h < v1; h += ln.slots) {
+            Unit<T, CH> u;
+            load_unit<T, CH, WIDE>(u, x + h * p.v.ld_head, ln.at);
+            store_unit<T, CH, WIDE>(out + h * p.cache.ld_head, ln.at, u);
         }
     }
 }
 
-template <class T, bool APPEND>
-cudaError_t launch_heads(HeadsParams &p, bool half, bool vec, int sm_count, cudaStream_t s) {
+template <class T, int CH, bool APPEND>
+cudaError_t launch_sized(HeadsParams &p, bool half, bool wide, int sm_count, cudaStream_t s) {
     const uint32_t n_all = p.q.n_heads + p.k.n_heads + p.v.n_heads;
     uint32_t lanes = 1;
-    while (lanes * 8 < p.head_dim) lanes *= 2;
-    const uint32_t slots = 128 / lanes;
-    // One pass over the heads per block while that leaves the GPU underfilled
-    // (each thread then carries one head), all heads of a token per block
-    // once there are enough tokens (the angles are formed once per block).
-    const uint64_t passes = (n_all + slots - 1) / slots;
-    const uint64_t room = (uint64_t)sm_count * 16;   // blocks of 128 resident
-    uint64_t per = (passes * p.n_tokens + room - 1) / room;
+    while (lanes * 2 * CH < p.head_dim) lanes *= 2;
+    // A warp takes one batch of heads while that leaves the GPU underfilled,
+    // all heads of a token once there are enough tokens (the angles are formed
+    // once per warp).
+    const uint32_t slots = 32 / lanes, batch = slots * kBatch;
+    const uint64_t batches = (n_all + batch - 1) / batch;
+    const uint64_t room = (uint64_t)sm_count * 32;   // warps resident
+    uint64_t per = (batches * p.n_tokens + room - 1) / room;
     if (per < 1) per = 1;
-    if (per > passes) per = passes;
-    p.heads_per_block = (uint32_t)per * slots;
-    const dim3 grid(p.n_tokens, (n_all + p.heads_per_block - 1) / p.heads_per_block);
+    if (per > batches) per = batches;
+    p.heads_per_group = (uint32_t)per * batch;
+    p.groups = (n_all + p.heads_per_group - 1) / p.heads_per_group;
+    const uint64_t blocks = ((uint64_t)p.n_tokens * p.groups + kWarps - 1) / kWarps;
+    if (blocks > 0x7fffffffu) return cudaErrorInvalidValue;
     if (half) {
-        if (vec) heads_kernel<T, true, APPEND, true><<<grid, 128, 0, s>>>(p);
-        else heads_kernel<T, true, APPEND, false><<<grid, 128, 0, s>>>(p);
+        if (wide) heads_kernel<T, CH, true, APPEND, true><<<(unsigned)blocks, kWarps * 32, 0, s>>>(p);
+        else heads_kernel<T, CH, true, APPEND, false><<<(unsigned)blocks, kWarps * 32, 0, s>>>(p);
     } else {
-        if (vec) heads_kernel<T, false, APPEND, true><<<grid, 128, 0, s>>>(p);
-        else heads_kernel<T, false, APPEND, false><<<grid, 128, 0, s>>>(p);
+        if (wide) heads_kernel<T, CH, false, APPEND, true><<<(unsigned)blocks, kWarps * 32, 0, s>>>(p);
+        else heads_kernel<T, CH, false, APPEND, false><<<(unsigned)blocks, kWarps * 32, 0, s>>>(p);
     }
     return cudaGetLastError();
+}
+
+// Chunks of 8 elements where the sizes allow it and, for f32, of 4.
+template <class T, bool APPEND>
+cudaError_t launch_heads(HeadsParams &p, bool half, bool wide, int sm_count, cudaStream_t s) {
+    if (sizeof(T) == 2 && wide && p.head_dim % 16 == 0 && p.half % 8 == 0)
+        return launch_sized<T, sizeof(T) == 2 ? 8 : 4, APPEND>(p, half, true, sm_count, s);
+    return launch_sized<T, 4, APPEND>(p, half, wide, sm_count, s);
 }
 
 int fail(const char *reason) {
@@ -272,9 +357,9 @@ HeadsView view_of(const tc_heads *h) {
     return {h->x, h->out, h->weight, h->ld_token, h->ld_head, h->ld_out_token, h->ld_out_head, h->n_heads};
 }
 
-// 4-element chunks of `item`-byte elements can move as one access.
+// Units of a row can be moved by 16-byte accesses.
 bool chunked(const void *p, uint64_t ld_token, uint64_t ld_head, uint32_t item) {
-    return !(reinterpret_cast<uintptr_t>(p) % (4 * item)) && !(ld_token % 4) && !(ld_head % 4);
+    return !(reinterpret_cast<uintptr_t>(p) % 16) && !(ld_token * item % 16) && !(ld_head * item % 16);
 }
 
 // Whether rows of `width` elements at the given strides share elements.
@@ -322,7 +407,6 @@ const char *take_rope(HeadsParams &p, const tc_rope *r, uint32_t head_dim, bool 
     half = r->layout == TC_ROPE_HALF;
     p.freq = r->freq;
     p.positions = r->positions;
-    p.rotary_units = r->rotary_dim / 8;
     p.half = r->rotary_dim / 2;
     p.n_axes = r->n_axes;
     p.amplitude = r->amplitude;

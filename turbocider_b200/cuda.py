@@ -546,21 +546,42 @@ def small_static_status(device: int = 0, clear: bool = True) -> int:
 # ------------------------------------------------------------ attention
 _ROPE_LAYOUTS = {"half": 0, "interleaved": 1}
 _ROPE_SCALINGS = {"plain": 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4}
-_dtype_ids: dict = {}
+_torch = None          # torch, its types and its stream query, looked up once: these calls are short
+
+
+def _torch_once():
+    global _torch
+    if _torch is None:
+        import torch
+
+        class T:
+            dtypes = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+            f32, f64, i32, dense = torch.float32, torch.float64, torch.int32, torch.contiguous_format
+            empty, empty_like = torch.empty, torch.empty_like
+            # address of a device's current stream without building a Stream object
+            raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+                lambda device: torch.cuda.current_stream(device).cuda_stream)
+        _torch = T
+    return _torch
 
 
 def _dtype_id(t) -> int:
-    if not _dtype_ids:
-        import torch
-        _dtype_ids.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
-    if t.dtype not in _dtype_ids:
+    i = _torch_once().dtypes.get(t.dtype)
+    if i is None:
         raise BackendError("tensors must be f32, f16 or bf16")
-    return _dtype_ids[t.dtype]
+    return i
+
+
+def _stream_of(ctx: Context, stream) -> int:
+    """Address of `stream`; None: the current stream of the context's device."""
+    if stream is None:
+        return _torch_once().raw_stream(ctx.device)
+    return getattr(stream, "cuda_stream", stream)
 
 
 def _ints(t, what: str, dims: int) -> int:
     """Address of a contiguous int32 device tensor."""
-    if str(t.dtype) != "torch.int32" or not t.is_cuda or t.dim() != dims or not t.is_contiguous():
+    if t.dtype is not _torch_once().i32 or not t.is_cuda or t.dim() != dims or not t.is_contiguous():
         raise BackendError(f"{what} must be a contiguous int32 device tensor of {dims} dimension(s)")
     return t.data_ptr()
 
@@ -591,21 +612,25 @@ class Rope:
     __slots__ = ("c", "freq", "positions")
 
     def __init__(self, freq, positions=None, layout: str = "half", sections=None, amplitude: float = 1.0):
-        if str(freq.dtype) != "torch.float64" or not freq.is_cuda or freq.dim() != 1 or not freq.is_contiguous():
+        if freq.dtype is not _torch_once().f64 or not freq.is_cuda or freq.dim() != 1 or not freq.is_contiguous():
             raise BackendError("freq must be a contiguous float64 device vector")
         if layout not in _ROPE_LAYOUTS:
             raise BackendError("invalid rotation layout")
-        axes = 1 if positions is None or positions.dim() == 1 else positions.shape[1]
-        sections = [freq.numel()] if sections is None else list(sections)
-        if axes != len(sections) or axes > 4:
+        axes, dims, pairs = 1, 1, freq.numel()
+        if positions is not None and positions.dim() == 2:
+            axes, dims = positions.shape[1], 2
+        if axes != (1 if sections is None else len(sections)) or not 1 <= axes <= 4:
             raise BackendError("one section for each of 1 to 4 position axes")
         self.freq, self.positions = freq, positions
         c = self.c = _Rope()
         c.freq = freq.data_ptr()
-        c.positions = None if positions is None else _ints(positions, "positions", positions.dim())
-        c.rotary_dim, c.layout, c.n_axes, c.amplitude = 2 * freq.numel(), _ROPE_LAYOUTS[layout], axes, amplitude
-        for i, n in enumerate(sections):
-            c.sections[i] = n
+        if positions is not None:
+            c.positions = _ints(positions, "positions", dims)
+        c.rotary_dim, c.layout, c.n_axes, c.amplitude = 2 * pairs, _ROPE_LAYOUTS[layout], axes, amplitude
+        if axes > 1:
+            c.sections = tuple(sections) + (0,) * (4 - axes)
+        elif sections is not None and sections[0] != pairs:
+            raise BackendError("the sections must add up to rotary_dim / 2")
 
 
 class PagedCache:
@@ -639,45 +664,45 @@ class PagedBatch:
     __slots__ = ("c", "tensors")
 
     def __init__(self, new_offsets, lengths, page_table, max_new: int, max_length: int):
-        n = lengths.numel()
-        if new_offsets.numel() != n + 1 or page_table.dim() != 2 or page_table.shape[0] != n:
+        n, shape, strides = lengths.numel(), page_table.shape, page_table.stride()
+        if len(shape) != 2 or shape[0] != n or new_offsets.numel() != n + 1:
             raise BackendError("new_offsets, lengths and page_table must have requests + 1, requests and requests rows")
-        if str(page_table.dtype) != "torch.int32" or not page_table.is_cuda or \
-                (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        if page_table.dtype is not _torch_once().i32 or not page_table.is_cuda or (strides[1] != 1 and shape[1] > 1):
             raise BackendError("page_table must be an int32 device tensor with contiguous rows")
         if max_new < 0 or max_length < 0:
             raise BackendError("max_new and max_length must not be negative")
         self.tensors = (new_offsets, lengths, page_table)
         c = self.c = _PagedBatch()
         c.new_offsets, c.lengths = _ints(new_offsets, "new_offsets", 1), _ints(lengths, "lengths", 1)
-        c.page_table, c.n_seq, c.table_width = page_table.data_ptr(), n, page_table.shape[1]
-        c.ld_table = page_table.stride(0) if n > 1 else page_table.shape[1]
+        c.page_table, c.n_seq, c.table_width = page_table.data_ptr(), n, shape[1]
+        c.ld_table = strides[0] if n > 1 else shape[1]
         c.max_new, c.max_length = max_new, max_length
 
 
-def _heads(x, out, weight, what: str):
-    """struct tc_heads of a [tokens, heads, head_dim] device tensor."""
-    if x.dim() != 3 or not x.is_cuda or (x.stride(2) != 1 and x.shape[2] > 1):
+def _heads(x, out, weight, what: str, fresh: bool = False):
+    """(struct tc_heads, out) of a [tokens, heads, head_dim] device tensor;
+    fresh: a contiguous result is allocated where out is None."""
+    shape, strides = x.shape, x.stride()
+    if len(shape) != 3 or not x.is_cuda or (strides[2] != 1 and shape[2] > 1):
         raise BackendError(f"{what} must be a device tensor [tokens, heads, head_dim] with a contiguous last dimension")
+    tokens, heads, dim = shape
     h = _Heads()
-    h.x, h.n_heads = x.data_ptr(), x.shape[1]
-    h.ld_token, h.ld_head = x.stride(0), x.stride(1)
+    h.x, h.n_heads, h.ld_token, h.ld_head = x.data_ptr(), heads, strides[0], strides[1]
     if out is not None:
-        if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or \
-                (out.stride(2) != 1 and out.shape[2] > 1):
+        strides = out.stride()
+        if out.shape != shape or out.dtype is not x.dtype or out.get_device() != x.get_device() or \
+                (strides[2] != 1 and dim > 1):
             raise BackendError(f"the result of {what} must have its shape, type and device")
-        h.out, h.ld_out_token, h.ld_out_head = out.data_ptr(), out.stride(0), out.stride(1)
+        h.out, h.ld_out_token, h.ld_out_head = out.data_ptr(), strides[0], strides[1]
+    elif fresh:
+        out = _torch.empty_like(x, memory_format=_torch.dense)
+        h.out, h.ld_out_token, h.ld_out_head = out.data_ptr(), heads * dim, dim
     if weight is not None:
-        if str(weight.dtype) != "torch.float32" or weight.shape != x.shape[2:] or not weight.is_contiguous() or \
-                weight.device != x.device:
+        if weight.dtype is not _torch.f32 or weight.dim() != 1 or weight.numel() != dim or \
+                not weight.is_contiguous() or weight.get_device() != x.get_device():
             raise BackendError("norm weights must be float32 device vectors of head_dim elements")
         h.weight = weight.data_ptr()
-    return h
-
-
-def _fresh(x):
-    """A contiguous tensor of x's shape, type and device."""
-    return x.new_empty(x.shape)
+    return h, out
 
 
 def qk_norm_rope(ctx: Context, q, k=None, rope: Rope | None = None, q_weight=None, k_weight=None,
@@ -686,18 +711,17 @@ def qk_norm_rope(ctx: Context, q, k=None, rope: Rope | None = None, q_weight=Non
     None: none) of query and key heads [tokens, heads, head_dim] in one
     launch.  Weights: f32 [head_dim].  q_out / k_out may be q / k.  Returns
     (q_out, k_out)."""
-    q_out = _fresh(q) if q_out is None else q_out
-    hq = _heads(q, q_out, q_weight, "q")
-    hk = None
+    dtype, hk = _dtype_id(q), None
+    hq, q_out = _heads(q, q_out, q_weight, "q", True)
+    tokens, _, dim = q.shape
     if k is not None:
-        if k.dtype != q.dtype or k.device != q.device or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+        if k.dtype is not q.dtype or k.get_device() != q.get_device() or k.shape[0] != tokens or k.shape[2] != dim:
             raise BackendError("q and k must share their type, device, tokens and head_dim")
-        k_out = _fresh(k) if k_out is None else k_out
-        hk = _heads(k, k_out, k_weight, "k")
-    if rope is not None and rope.positions is not None and rope.positions.shape[0] != q.shape[0]:
+        hk, k_out = _heads(k, k_out, k_weight, "k", True)
+    if rope is not None and rope.positions is not None and rope.positions.shape[0] != tokens:
         raise BackendError("one position for each token")
-    _check(lib().tc_cuda_qk_norm_rope(ctx.handle, hq, hk, q.shape[0], q.shape[2], _dtype_id(q), int(eps is not None),
-                                      eps or 0.0, None if rope is None else rope.c, _stream_ptr(stream)))
+    _check(lib().tc_cuda_qk_norm_rope(ctx.handle, hq, hk, tokens, dim, dtype, eps is not None, eps or 0.0,
+                                      None if rope is None else rope.c, _stream_of(ctx, stream)))
     return q_out, k_out
 
 
@@ -706,20 +730,20 @@ def kv_append(ctx: Context, cache: PagedCache, batch: PagedBatch, k, v, rope: Ro
     """Writes the step's keys (normed with eps not None, rotated with rope)
     and values [tokens, heads, head_dim] to the cache and, in the same launch,
     norms and rotates the queries.  Returns q_out (None without q)."""
-    if k.dtype != cache.dtype or v.dtype != cache.dtype or k.shape != v.shape or k.shape[2] != cache.head_dim:
+    shape = k.shape
+    if k.dtype is not cache.dtype or v.dtype is not cache.dtype or v.shape != shape or shape[2] != cache.head_dim:
         raise BackendError("keys and values must have the cache's type and head_dim")
-    if rope is not None and rope.positions is not None and rope.positions.shape[0] != k.shape[0]:
+    tokens, hq = shape[0], None
+    if rope is not None and rope.positions is not None and rope.positions.shape[0] != tokens:
         raise BackendError("one position for each token")
-    hq = None
     if q is not None:
-        if q.dtype != cache.dtype or q.shape[0] != k.shape[0] or q.shape[2] != cache.head_dim:
+        if q.dtype is not cache.dtype or q.shape[0] != tokens or q.shape[2] != shape[2]:
             raise BackendError("queries must have the cache's type and head_dim and one row for each key")
-        q_out = _fresh(q) if q_out is None else q_out
-        hq = _heads(q, q_out, q_weight, "q")
-    batch.c.n_tokens = k.shape[0]
-    _check(lib().tc_cuda_kv_append(ctx.handle, cache.c, batch.c, _heads(k, None, k_weight, "k"),
-                                   _heads(v, None, None, "v"), hq, int(eps is not None), eps or 0.0,
-                                   None if rope is None else rope.c, _stream_ptr(stream)))
+        hq, q_out = _heads(q, q_out, q_weight, "q", True)
+    batch.c.n_tokens = tokens
+    _check(lib().tc_cuda_kv_append(ctx.handle, cache.c, batch.c, _heads(k, None, k_weight, "k")[0],
+                                   _heads(v, None, None, "v")[0], hq, eps is not None, eps or 0.0,
+                                   None if rope is None else rope.c, _stream_of(ctx, stream)))
     return q_out if q is not None else None
 
 
@@ -729,23 +753,25 @@ def paged_attention(ctx: Context, cache: PagedCache, batch: PagedBatch, q, scale
     over each request's cache (scale None: head_dim ** -0.5); query heads share
     cache heads in equal groups.  window > 0: only positions nearer than that.
     Returns out, or (out, lse) with lse f32 [tokens, heads]."""
-    import torch
-    if q.dim() != 3 or q.dtype != cache.dtype or q.device != cache.k.device or q.shape[2] != cache.head_dim or \
-            q.stride(2) != 1:
+    t = _torch_once()
+    shape, strides = q.shape, q.stride()
+    if len(shape) != 3 or q.dtype is not cache.dtype or q.get_device() != cache.k.get_device() or \
+            shape[2] != cache.head_dim or strides[2] != 1:
         raise BackendError("queries must be [tokens, heads, head_dim] of the cache's type, device and head_dim")
-    if out is None:
-        out = _fresh(q)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(2) != 1:
-        raise BackendError("the result must have the queries' shape, type and device")
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
     a = _Attention()
-    a.q, a.out, a.lse = q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else None
-    a.ld_q_token, a.ld_q_head = q.stride(0), q.stride(1)
-    a.ld_out_token, a.ld_out_head = out.stride(0), out.stride(1)
-    a.n_heads, a.causal, a.window = q.shape[1], int(causal), window
-    a.scale = q.shape[2] ** -0.5 if scale is None else scale
-    batch.c.n_tokens = q.shape[0]
-    _check(lib().tc_cuda_paged_attention(ctx.handle, cache.c, batch.c, a, _stream_ptr(stream)))
+    a.q, a.ld_q_token, a.ld_q_head, a.n_heads = q.data_ptr(), strides[0], strides[1], shape[1]
+    if out is None:
+        out = t.empty_like(q, memory_format=t.dense)
+    strides = out.stride()
+    if out.shape != shape or out.dtype is not q.dtype or out.get_device() != q.get_device() or strides[2] != 1:
+        raise BackendError("the result must have the queries' shape, type and device")
+    a.out, a.ld_out_token, a.ld_out_head = out.data_ptr(), strides[0], strides[1]
+    if return_lse:
+        lse = t.empty(shape[:2], dtype=t.f32, device=q.device)
+        a.lse = lse.data_ptr()
+    a.causal, a.window, a.scale = causal, window, shape[2] ** -0.5 if scale is None else scale
+    batch.c.n_tokens = shape[0]
+    _check(lib().tc_cuda_paged_attention(ctx.handle, cache.c, batch.c, a, _stream_of(ctx, stream)))
     return (out, lse) if return_lse else out
 
 
