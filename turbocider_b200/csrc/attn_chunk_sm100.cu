@@ -3,33 +3,42 @@
 //
 // A CTA takes 256 rows (the query heads of one cache head packed with the
 // tokens, see attn_paged.cu) as two 128-row tiles and walks the keys that they
-// see in steps of 128:
+// see in steps of 128, each tile in half-steps of 64:
 //   S_i = Q_i K^T           tcgen05.mma, both operands in shared memory, S in TMEM
 //   P_i = 2^(c S_i - c m)   one thread per row (two warpgroups, one per tile)
 //   O_i += P_i V            tcgen05.mma, P_i in TMEM (over S_i), V in shared
 //                           memory as it lies in the cache (MN-major operand)
-// Four 128 x 128 x 128 products a step (2048 tensor cycles at head_dim 128)
-// against 32768 exponentials (2048 cycles of the special-function units), so
-// the tile not being exponentiated keeps the tensor cores busy: the issuing
-// thread orders PV_0(j), S_0(j+1), PV_1(j), S_1(j+1), and a commit behind
-// S_i(j+1) also covers PV_i(j), so the warpgroup that finds S_i(j+1) complete
-// may rescale O_i itself.  That happens only when a row's maximum has grown by
-// more than 2^8 since the last time (P then stays below 256, exact enough in
-// either 16-bit type), i.e. seldom after the first steps.
+// S_i has a buffer for each half, so its warpgroup goes from one half-step to
+// the next without waiting for a product: while it works on one half, the
+// tile's issuing warp adds the other to O_i and refills its buffer.  O_i is
+// rescaled only when a row's maximum has grown by more than 2^8 since the last
+// time (P then stays below 256, exact enough in either 16-bit type), i.e.
+// seldom after the first steps, by the warpgroup itself once the product before
+// has finished.  The rounding of P to the cache's type is the only one before
+// the result's; sums are taken before it.
 //
 //   warps 0-3, 4-7   softmax of tile 0 / 1, epilogue
-//   warp 8           TMA producer: K and V tiles of 128 keys through a ring of
+//   warps 8, 9       MMA issue of tile 0 / 1; warp 8 allocates TMEM
+//   warp 10          TMA producer: K and V tiles of 128 keys through a ring of
 //                    stages, one box per page piece and 64-element half, the
 //                    boxes of a tile issued by the warp's lanes in parallel
-//   warps 10, 11     nothing (they complete the warpgroup that gives up registers)
-//   warp 9           TMEM allocation, MMA issue; zeroes the rows of V outside
-//                    the keys seen in the first and last step (their bytes are
-//                    whatever the page holds there, and 0 * NaN is NaN)
+//   warp 11          clears the rows of V that no row sees
 //
-// TMEM: S_0, S_1 (128 columns each), O_0, O_1 (head_dim each).  Blocks of rows
-// go heaviest first (last rows first).  With few blocks the keys are split
-// over CTAs: partial results (column-major, so that the 128 threads of a tile
-// store and load whole lines) and the last to finish joins them in order.
+// TMEM: S_0, S_1 (two halves of 64 columns each), O_0, O_1 (head_dim each).
+// Blocks of rows go heaviest first (last rows first).  With few blocks the keys
+// are split over CTAs: partial results (column-major, so that the 128 threads of
+// a tile store and load whole lines) and the last to finish joins them in order.
+//
+// What bounds it: the GPU's 1000 W.  2 x 4224 image tokens, 30 heads of 128, f16:
+// 557 us (985 TFLOP/s) in the first milliseconds, 614 us (892 TFLOP/s; 66 % of
+// what cuBLAS sustains) in a loop, where the cap lowers the clock from 1965 to
+// about 1700 MHz.  At full clock a step takes about 4500 cycles against 2048 of
+// the tensor cores and 2048 of the special-function units (exponentials): two
+// softmax warps per scheduler reach 10 of them in 100 cycles, not 12.5.
+// Tried and dropped: 128-key softmax steps with one issuer (3 % slower on
+// prompts, 3 % faster on long chunks), two threads per row, tiles taking turns
+// with the special-function units, a quarter of the exponentials by polynomial
+// (each 2 to 10 % slower on long chunks: more instructions, more power).
 //
 // Every wait is bounded; on timeout the kernel sets TC_STATUS_TIMEOUT, drains
 // its copies and MMAs, frees TMEM and returns.  No multicast.
@@ -39,11 +48,6 @@ namespace tc {
 namespace {
 
 constexpr int kThreads = 384;
-// Registers of a thread: 384 threads launch with 168; the warpgroup of the
-// producer and the issuer gives up what the softmax warpgroups (which hold 128
-// scores) take.
-constexpr int kSoftmaxRegs = 216, kOtherRegs = 72, kLaunchRegs = 168;
-static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * kLaunchRegs, "the shares exceed the launch's registers");
 constexpr float kLazy = 8.f;   // log2 of the growth of a maximum that is let pass
 
 template <int DP>
@@ -54,28 +58,36 @@ struct ChunkLayout {
     static constexpr uint32_t stages = DP == 128 ? 5 : 8;
     static constexpr uint32_t q_off = 0, kv_off = 2 * tile_bytes;
     static constexpr uint32_t bar_off = kv_off + stages * tile_bytes;
-    // kv_full[S] kv_empty[S] s_full[2] p_full[2] o_full[2] q_full fin
-    static constexpr uint32_t misc_off = bar_off + (2 * stages + 8) * 8;
+    // kv_full[S] kv_empty[S], [tile][half]: s_full p_full pv_done, then q_full fin v_fixed[2]
+    static constexpr uint32_t misc_off = bar_off + (2 * stages + 16) * 8;
     static constexpr uint32_t bytes = misc_off + 16 + 1024;
     static constexpr uint32_t s_col = 0, o_col = 256, tmem_cols = 512;
     static_assert(bytes <= 232448, "shared memory per CTA exceeds the sm_100 limit");
 };
 
-// bar_wait without a call (a call would fix the caller's registers below the
-// softmax warpgroups' share).
-__device__ __forceinline__ bool wait(uint32_t b, uint32_t parity, volatile uint32_t *abort_flag, uint32_t *status,
-                                     bool honor_abort = true) {
-    if (bar_try(b, parity)) return true;
-    const uint64_t t0 = gtimer();
-    for (;;) {
-        if (bar_try_sleep(b, parity, 20000u)) return true;
-        if (honor_abort && *abort_flag) return false;
-        if (gtimer() - t0 > kTimeoutNs) {
-            atomicOr(status, kStatusTimeout);
-            *abort_flag = 1u;
-            return false;
-        }
-    }
+// Bounded wait of a warp, a few instructions: a wait that gives up (after about
+// a second) returns false; the role then ends, and those that wait for it give
+// up in turn.  Every phase of a barrier must be waited for, or be known to be
+// the current one: a parity two phases back looks the same.
+__device__ __forceinline__ bool wait(uint32_t b, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p, q;\n .reg .u32 n;\n mov.u32 n, 20000;\n"
+        "again_%=:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n @p bra done_%=;\n"
+        " sub.u32 n, n, 1;\n setp.ne.u32 q, n, 0;\n @q bra again_%=;\n"
+        "done_%=:\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok) : "r"(b), "r"(parity), "r"(50000u) : "memory");
+    return __all_sync(0xffffffffu, ok != 0);
+}
+// One arrival for the warp.
+__device__ __forceinline__ void warp_arrive(uint32_t b) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) bar_arrive(b);
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t ok;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok));
+    return ok != 0;
 }
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -105,6 +117,49 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *v) {
           "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
         : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float *v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15}, [%16];"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+          "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16};"
+        ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+          "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+
+// pk = 16-bit 2^(c s + off) of N scores, sums added to `sum`.
+template <bool BF16, int N>
+__device__ __forceinline__ void exps(const float *s, uint64_t c2, uint64_t off2, uint32_t *pk, uint64_t (&sum)[2]) {
+#pragma unroll
+    for (int k = 0; k < N; k += 2) {
+        float e0, e1;
+        f2unpack(f2fma(f2pack(__float_as_uint(s[k]), __float_as_uint(s[k + 1])), c2, off2), e0, e1);
+        e0 = ex2(e0);
+        e1 = ex2(e1);
+        pk[k / 2] = pack16<BF16>(e0, e1);
+        sum[(k / 2) & 1] = f2add(sum[(k / 2) & 1], f2pack(__float_as_uint(e0), __float_as_uint(e1)));
+    }
+}
+
+// Largest of 64 scores (NaN passed over).
+__device__ __forceinline__ float top_of(const float *s) {
+    float m[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+    for (int k = 4; k < 60; k += 8)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) asm("max.f32 %0, %0, %1, %2;" : "+f"(m[e]) : "f"(s[k + e]), "f"(s[k + 4 + e]));
+    asm("max.f32 %0, %0, %1, %2;" : "+f"(m[0]) : "f"(s[60]), "f"(s[61]));
+    asm("max.f32 %0, %0, %1, %2;" : "+f"(m[1]) : "f"(s[62]), "f"(s[63]));
+    return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+}
+
 // A in TMEM, B in shared memory.
 __device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
@@ -130,9 +185,15 @@ struct Work {
     uint32_t b, h, part, group_index, n_split, split;
     int32_t row0, n_rows;
     int32_t lo[2], hi[2];     // keys that tile i's rows see, within the CTA's share
-    int32_t first[2], last[2];   // its steps (tile i has none: first == last)
+    int32_t first[2], last[2];   // its half-steps of 64 keys (tile i has none: first == last)
     int32_t begin, end;       // steps of the CTA (keys 128 step ..)
+    int32_t seen_lo, seen_hi; // keys that any row sees, within the share
 };
+
+// Step j has keys that no row sees (only the first and the last can).
+__device__ __forceinline__ bool cut_step(const Work &w, int32_t j) {
+    return j * kChunkKeys < w.seen_lo || (j + 1) * kChunkKeys > w.seen_hi;
+}
 
 __device__ __forceinline__ bool find_work(const AttnParams &p, Work &w) {
     uint32_t id = blockIdx.x;
@@ -187,12 +248,14 @@ __device__ __forceinline__ bool find_work(const AttnParams &p, Work &w) {
         w.lo[i] = max(w.lo[i], w.begin * kChunkKeys);
         w.hi[i] = min(w.hi[i], w.end * kChunkKeys);
         if (w.hi[i] <= w.lo[i]) {
-            w.first[i] = w.last[i] = w.begin;
+            w.first[i] = w.last[i] = 2 * w.begin;
         } else {
-            w.first[i] = w.lo[i] / kChunkKeys;
-            w.last[i] = (w.hi[i] + kChunkKeys - 1) / kChunkKeys;
+            w.first[i] = w.lo[i] / 64;
+            w.last[i] = (w.hi[i] + 63) / 64;
         }
     }
+    w.seen_lo = min(w.first[0] < w.last[0] ? w.lo[0] : 0x7fffffff, w.first[1] < w.last[1] ? w.lo[1] : 0x7fffffff);
+    w.seen_hi = max(w.hi[0], w.hi[1]);
     w.group_index = blk * p.n_kv + w.h;
     w.part = w.group_index * p.splits + w.split;
     return true;
@@ -227,36 +290,39 @@ __global__ void __launch_bounds__(kThreads, 1)
     using L = ChunkLayout<DP>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    // Warps of the block in the order of their roles: the issuing warp is the
+    // block's first, since the scheduler favours the oldest of the ready warps
+    // (as the last it waited about 500 cycles for its turn at every barrier).
+    const uint32_t warp = (threadIdx.x / 32 + 8) % 12, lane = threadIdx.x % 32, tid = warp * 32 + lane;
     Work w;
     if (!find_work(p, w)) return;
     const uint32_t bars = su32(smem + L::bar_off);
     auto kv_full = [&](uint32_t i) { return bars + 8 * i; };
     auto kv_empty = [&](uint32_t i) { return bars + 8 * (L::stages + i); };
-    auto s_full = [&](uint32_t i) { return bars + 8 * (2 * L::stages + i); };
-    auto p_full = [&](uint32_t i) { return bars + 8 * (2 * L::stages + 2 + i); };
-    auto o_full = [&](uint32_t i) { return bars + 8 * (2 * L::stages + 4 + i); };
-    const uint32_t q_full = bars + 8 * (2 * L::stages + 6), fin = q_full + 8;
+    auto s_full = [&](uint32_t i, uint32_t h) { return bars + 8 * (2 * L::stages + 2 * i + h); };
+    auto p_full = [&](uint32_t i, uint32_t h) { return bars + 8 * (2 * L::stages + 4 + 2 * i + h); };
+    auto pv_done = [&](uint32_t i, uint32_t h) { return bars + 8 * (2 * L::stages + 8 + 2 * i + h); };
+    const uint32_t q_full = bars + 8 * (2 * L::stages + 12), fin = q_full + 8, v_fixed = fin + 8;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + L::misc_off);
-    volatile uint32_t *abort_flag = tmem_slot + 1;
-    uint32_t *last_flag = tmem_slot + 2;
+    uint32_t *last_flag = tmem_slot + 1;
 
-    if (threadIdx.x == 0) {
+    if (tid == 0) {
         for (uint32_t i = 0; i < L::stages; ++i) {
             bar_init(kv_full(i), 1);
-            bar_init(kv_empty(i), 1);
+            bar_init(kv_empty(i), 3);
         }
-        for (int i = 0; i < 2; ++i) {
-            bar_init(s_full(i), 1);
-            bar_init(p_full(i), 128);
-            bar_init(o_full(i), 1);
+        for (uint32_t k = 0; k < 4; ++k) {
+            bar_init(s_full(k / 2, k % 2), 1);
+            bar_init(p_full(k / 2, k % 2), 4);
+            bar_init(pv_done(k / 2, k % 2), 1);
         }
-        bar_init(q_full, 256);
-        bar_init(fin, 1);
-        *abort_flag = 0u;
+        bar_init(q_full, 8);
+        bar_init(fin, 2);
+        bar_init(v_fixed, 1);
+        bar_init(v_fixed + 8, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 9) {
+    if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                      ::"r"(su32(tmem_slot)), "r"(L::tmem_cols));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -267,13 +333,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem = *tmem_slot;
 
     if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-        if (warp == 8) {
+        if (warp == 10) {
         // ---------------------------------------------------- TMA producer
         const uint32_t box = min((uint32_t)kChunkKeys, 1u << p.page_shift), pieces = kChunkKeys / box;
         const uint32_t piece = lane % pieces, half0 = lane / pieces;   // lanes: 32 / pieces halves at a time
-        const int32_t key_end = max(w.hi[0], w.hi[1]);
+        const int32_t key_end = w.seen_hi;
         uint32_t st = 0, ph = 0, issued = 0;
+        bool ok = true;
         for (int32_t j = w.begin; j < w.end; ++j) {
             // this lane's page piece of the step
             const int32_t pos = j * kChunkKeys + (int32_t)(piece * box);
@@ -282,11 +348,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (on) page = max(load_page(p.batch, p.n_pages, w.b, (uint32_t)pos >> p.page_shift, p.status), 0);
             const int token = (int)((uint32_t)pos & ((1u << p.page_shift) - 1));
             const uint32_t n_on = min(pieces, (uint32_t)(key_end - j * kChunkKeys + (int32_t)box - 1) / box);
-            bool ok = true;
-#pragma unroll
+#pragma unroll 1
             for (int kv = 0; kv < 2; ++kv) {
-                ok = wait(kv_empty(st), ph ^ 1, abort_flag, p.status);
-                if (!(ok = __all_sync(0xffffffffu, ok))) break;
+                if (!(ok = wait(kv_empty(st), ph ^ 1))) break;
                 if (lane == 0) bar_expect_tx(kv_full(st), n_on * box * DP * 2);
                 __syncwarp();
                 const uint32_t dst = su32(smem + L::kv_off + st * L::tile_bytes) + piece * box * 128;
@@ -300,115 +364,124 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!ok) break;
         }
         __syncwarp();
-        if (lane == 0)
-            // every copy issued has landed before exit
-            for (uint32_t n = issued > L::stages ? issued - L::stages : 0; n < issued; ++n)
-                wait(kv_full(n % L::stages), (n / L::stages) & 1u, abort_flag, p.status, false);
+        // every copy issued has landed before exit
+        for (uint32_t n = issued > L::stages ? issued - L::stages : 0; n < issued; ++n)
+            ok = wait(kv_full(n % L::stages), (n / L::stages) & 1u) && ok;
+        if (!ok && lane == 0) atomicOr(p.status, kStatusTimeout);
         __syncwarp();
-        } else if (warp == 9) {
-        // ---------------------------------------------------- MMA issuer
-        constexpr uint32_t idesc_s = mma_idesc<128, !BF16>();
+        } else if (warp == 8 || warp == 9) {
+        // ---------------------------------------------------- MMA issuers, one per tile
+        // (the whole warp runs the loop, so that descriptors and bounds stay
+        // uniform; one elected lane issues)
+        constexpr uint32_t idesc_s = mma_idesc<64, !BF16>();
         constexpr uint32_t idesc_o = mma_idesc<DP, !BF16>() | (1u << 16);   // B is MN-major
-        const uint32_t q_addr = su32(smem + L::q_off), kv_addr = su32(smem + L::kv_off);
+        constexpr uint32_t kHalfKeys = 64 * 128 >> 4;                       // 64 keys on, in descriptor units
+        auto uniform = [](int32_t v) { return __shfl_sync(0xffffffffu, v, 0); };
+        const uint32_t i = uniform(warp - 8);
+        const int32_t begin = uniform(w.begin), end = uniform(w.end);
+        const int32_t first = uniform(i ? w.first[1] : w.first[0]), last = uniform(i ? w.last[1] : w.last[0]);
+        const uint32_t q_low = desc_low(su32(smem + L::q_off) + i * L::tile_bytes, 1);
+        const uint32_t k_low = desc_low(su32(smem + L::kv_off), 1);
+        const uint32_t v_low = desc_low(su32(smem + L::kv_off), L::half_bytes >> 4);
+        const uint32_t s_tmem = tmem + L::s_col + i * 128, o_tmem = tmem + L::o_col + i * DP;
         // ring positions of K and V of step j: 2 (j - begin) and one more
         auto stage_of = [&](uint32_t n) { return n % L::stages; };
-        auto phase_of = [&](uint32_t n) { return (n / L::stages) & 1u; };
-        auto wait_kv = [&](uint32_t n) {
-            return __all_sync(0xffffffffu, wait(kv_full(stage_of(n)), phase_of(n), abort_flag, p.status));
-        };
-        const uint32_t q_low = desc_low(q_addr, 1), k_low = desc_low(kv_addr, 1);
-        const uint32_t v_low = desc_low(kv_addr, L::half_bytes >> 4);
-        auto issue_s = [&](int i, uint32_t n) {
-            if (lane == 0) {
-                const uint32_t q = q_low + i * (L::tile_bytes >> 4), k = k_low + stage_of(n) * (L::tile_bytes >> 4);
-#pragma unroll
-                for (uint32_t kk = 0; kk < DP / 16; ++kk) {
-                    const uint32_t off = ((kk / 4) * L::half_bytes + (kk % 4) * 32) >> 4;
-                    mma_f16(tmem + L::s_col + i * 128, desc(q + off), desc(k + off), idesc_s, kk ? 1u : 0u);
-                }
-                mma_commit(s_full(i));
-            }
-        };
-        const int32_t seen_lo = min(w.first[0] < w.last[0] ? w.lo[0] : 0x7fffffff,
-                                    w.first[1] < w.last[1] ? w.lo[1] : 0x7fffffff);
-        const int32_t seen_hi = max(w.hi[0], w.hi[1]);
-        bool ok = __all_sync(0xffffffffu, wait(q_full, 0, abort_flag, p.status));
+        auto wait_kv = [&](uint32_t n) { return wait(kv_full(stage_of(n)), (n / L::stages) & 1u); };
+        bool ok = wait(q_full, 0);
         tc_fence_after();
-        uint32_t n = 0;   // ring position of K(j)
-        if (ok && w.begin < w.end) {
-            ok = wait_kv(0);
-            tc_fence_after();
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-                if (ok && w.first[i] == w.begin && w.first[i] < w.last[i]) issue_s(i, 0);
-            if (ok && lane == 0) mma_commit(kv_empty(0));
-        }
-        for (int32_t j = w.begin; ok && j < w.end; ++j, n += 2) {
-            ok = wait_kv(n + 1);
-            const int32_t key0 = j * kChunkKeys;
-            if (ok && (key0 < seen_lo || key0 + kChunkKeys > seen_hi)) {
-                const uint32_t v = kv_addr + stage_of(n + 1) * L::tile_bytes;
-                // rows [0, below) and [above, 128), whole 16-byte pieces
-                const uint32_t below = (uint32_t)min(max(seen_lo - key0, 0), kChunkKeys);
-                const uint32_t above = (uint32_t)min(max(seen_hi - key0, 0), kChunkKeys);
-                for (uint32_t c = lane; c < (below + kChunkKeys - above) * (DP / 8); c += 32) {
-                    const uint32_t rr = c / 8 / L::halves, hf = c / 8 % L::halves;
-                    const uint32_t r = rr < below ? rr : above + rr - below;
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};"
-                                 ::"r"(v + hf * L::half_bytes + r * 128 + (c % 8) * 16), "r"(0) : "memory");
-                }
-                fence_proxy_async();
-                __syncwarp();
+        // Round j: for each half of the keys, O += P(j - 1) V(j - 1), then S(j)
+        // over the probabilities just used.  Every K and V of the CTA is
+        // released by both issuers and the clearing warp.
+        for (int32_t j = begin; ok && j <= end; ++j) {
+            const uint32_t n = 2 * (uint32_t)(j - begin);
+            if (j > begin) {
+                if (!(ok = wait_kv(n - 1))) break;
+                if (cut_step(w, j - 1) && !(ok = wait(v_fixed + (j - 1 > begin ? 8 : 0), 0))) break;
             }
-            bool waited = false;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if (!ok) break;
-                if (j >= w.first[i] && j < w.last[i]) {
-                    ok = __all_sync(0xffffffffu,
-                                    wait(p_full(i), (uint32_t)(j - w.first[i]) & 1u, abort_flag, p.status));
-                    if (!ok) break;
+            const uint32_t v = v_low + stage_of(n - 1) * (L::tile_bytes >> 4);
+            const uint32_t k = k_low + stage_of(n) * (L::tile_bytes >> 4);
+#pragma unroll 1
+            for (uint32_t h = 0; h < 2; ++h) {
+                // half-steps of the product and of the scores, and how many came before
+                const int32_t gp = 2 * (j - 1) + (int32_t)h, gs = gp + 2;
+                const uint32_t done = (uint32_t)(gp - first);
+                if (gp >= first && gp < last) {
+                    if (!(ok = wait(p_full(i, h), done >> 1 & 1u))) break;
                     tc_fence_after();
-                    if (lane == 0) {
-                        const uint32_t v = v_low + stage_of(n + 1) * (L::tile_bytes >> 4);
+                    if (elect_one()) {
 #pragma unroll
-                        for (uint32_t kk = 0; kk < kChunkKeys / 16; ++kk)
-                            mma_f16_ts(tmem + L::o_col + i * DP, tmem + L::s_col + i * 128 + kk * 8,
-                                       desc(v + kk * (2048 >> 4)), idesc_o, j > w.first[i] || kk ? 1u : 0u);
-                        if (j + 1 == w.last[i]) mma_commit(o_full(i));
+                        for (uint32_t kk = 0; kk < 4; ++kk)
+                            mma_f16_ts(o_tmem, s_tmem + h * 64 + kk * 8, desc(v + h * kHalfKeys + kk * (2048 >> 4)),
+                                       idesc_o, kk ? 1u : (uint32_t)(done > 0));
+                        mma_commit(pv_done(i, h));
                     }
+                    __syncwarp();
                 }
-                if (j + 1 >= w.first[i] && j + 1 < w.last[i]) {
-                    if (!waited) {
-                        ok = wait_kv(n + 2);
-                        if (!ok) break;
-                        tc_fence_after();
-                        waited = true;
+                if (h == 0 && j < end && !(ok = wait_kv(n))) break;
+                if (gs >= first && gs < last) {
+                    tc_fence_after();
+                    if (elect_one()) {
+#pragma unroll
+                        for (uint32_t kk = 0; kk < DP / 16; ++kk) {
+                            const uint32_t off = ((kk / 4) * L::half_bytes + (kk % 4) * 32) >> 4;
+                            mma_f16(s_tmem + h * 64, desc(q_low + off), desc(k + h * kHalfKeys + off), idesc_s,
+                                    kk ? 1u : 0u);
+                        }
+                        mma_commit(s_full(i, h));
                     }
-                    issue_s(i, n + 2);
+                    __syncwarp();
                 }
             }
-            if (ok && j + 1 < w.end && !waited) ok = wait_kv(n + 2);
-            if (ok && lane == 0) {
-                mma_commit(kv_empty(stage_of(n + 1)));
-                if (j + 1 < w.end) mma_commit(kv_empty(stage_of(n + 2)));
+            if (ok && elect_one()) {
+                if (j > begin) mma_commit(kv_empty(stage_of(n - 1)));
+                if (j < end) mma_commit(kv_empty(stage_of(n)));
             }
+            __syncwarp();
         }
-        if (lane == 0) {
-            mma_commit(fin);   // every MMA issued has completed before TMEM is freed
-            wait(fin, 0, abort_flag, p.status, false);
+        if (elect_one()) mma_commit(fin);   // every MMA issued has completed before TMEM is freed
+        __syncwarp();
+        ok = wait(fin, 0) && ok;
+        if (!ok && lane == 0) atomicOr(p.status, kStatusTimeout);
+        } else if (warp == 11) {
+        // ---------------------------------------------------- values that no row sees
+        // Rows of V outside the keys seen are cleared before the product reads
+        // them: their bytes are whatever the page holds there, and 0 * NaN is NaN.
+        // The warp sees every load of the ring and its release with the issuers'
+        // (a wait that skipped phases could not tell one from the next but one).
+        const int32_t seen_lo = w.seen_lo, seen_hi = w.seen_hi;
+        const uint32_t loads = 2 * (uint32_t)(w.end - w.begin);
+        for (uint32_t n = 0; n < loads; ++n) {
+            if (!wait(kv_full(n % L::stages), (n / L::stages) & 1u)) break;
+            const int32_t j = w.begin + (int32_t)(n / 2);
+            if (n % 2 == 0 || !cut_step(w, j)) {
+                warp_arrive(kv_empty(n % L::stages));
+                continue;
+            }
+            const uint32_t v = su32(smem + L::kv_off) + (n % L::stages) * L::tile_bytes;
+            const int32_t key0 = j * kChunkKeys;
+            // rows [0, below) and [above, 128), whole 16-byte pieces
+            const uint32_t below = (uint32_t)min(max(seen_lo - key0, 0), kChunkKeys);
+            const uint32_t above = (uint32_t)min(max(seen_hi - key0, 0), kChunkKeys);
+            for (uint32_t c = lane; c < (below + kChunkKeys - above) * (DP / 8); c += 32) {
+                const uint32_t rr = c / 8 / L::halves, hf = c / 8 % L::halves;
+                const uint32_t r = rr < below ? rr : above + rr - below;
+                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};"
+                             ::"r"(v + hf * L::half_bytes + r * 128 + (c % 8) * 16), "r"(0) : "memory");
+            }
+            fence_proxy_async();
+            warp_arrive(v_fixed + (j > w.begin ? 8 : 0));
+            warp_arrive(kv_empty(n % L::stages));
         }
         __syncwarp();
         }
     } else {
         // ---------------------------------------------------- softmax
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         const int i = warp / 4;
         const int32_t first = i ? w.first[1] : w.first[0], last = i ? w.last[1] : w.last[0];
         // queries of both tiles: DP / 8 16-byte pieces a row, all 256 threads
         {
             constexpr uint32_t per = DP / 8;
-            for (uint32_t c = threadIdx.x; c < 256 * per; c += 256) {
+            for (uint32_t c = tid; c < 256 * per; c += 256) {
                 const uint32_t r = c / per, x = c % per;
                 const int32_t row = w.row0 + (int32_t)r;
                 uint32_t v[4] = {};
@@ -432,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                              ::"r"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
             }
             fence_proxy_async();
-            bar_arrive(q_full);
+            warp_arrive(q_full);
         }
         const uint32_t quad = warp & 3, r = quad * 32 + lane;     // row of the tile = TMEM lane
         const uint32_t t_s = tmem + ((quad * 32) << 16) + L::s_col + i * 128;
@@ -445,76 +518,59 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float c = p.scale_log2;
         float m = -INFINITY, l = 0.f;   // running maximum (of S), sum
         bool ok = true;
-        for (int32_t j = first; j < last; ++j) {
-            ok = wait(s_full(i), (uint32_t)(j - first) & 1u, abort_flag, p.status);
-            if (!(ok = __all_sync(0xffffffffu, ok))) break;
+        // half-steps of 64 keys
+        for (int32_t g = first; g < last; ++g) {
+            const uint32_t h = g & 1, done = (uint32_t)(g - first), parity = done >> 1 & 1u;
+            if (!(ok = wait(s_full(i, h), parity))) break;
             tc_fence_after();
-            float s[128];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) tmem_ld32_nowait(t_s + 32 * k, s + 32 * k);
+            float s[64];
+            tmem_ld32_nowait(t_s + h * 64, s);
+            tmem_ld32_nowait(t_s + h * 64 + 32, s + 32);
             tmem_wait_ld();
-            const int32_t a = lo - j * kChunkKeys, z = hi - j * kChunkKeys;   // seen: a <= column < z
-            if (__any_sync(0xffffffffu, a > 0 || z < kChunkKeys)) {
+            const int32_t a = lo - g * 64, z = hi - g * 64;   // seen: a <= k < z
+            if (__builtin_expect(__any_sync(0xffffffffu, a > 0 || z < 64), 0)) {
 #pragma unroll
-                for (int k = 0; k < 128; ++k)
+                for (int k = 0; k < 64; ++k)
                     if (k < a || k >= z) s[k] = -INFINITY;
             }
-            float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-            for (int k = 4; k < 128; k += 4) {
-                mx[0] = fmaxf(mx[0], s[k]);
-                mx[1] = fmaxf(mx[1], s[k + 1]);
-                mx[2] = fmaxf(mx[2], s[k + 2]);
-                mx[3] = fmaxf(mx[3], s[k + 3]);
-            }
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            const float top = top_of(s);
             const bool grow = m == -INFINITY ? top > m : (top - m) * c > kLazy;
-            if (__any_sync(0xffffffffu, grow)) {
+            if (__builtin_expect(__any_sync(0xffffffffu, grow), 0)) {
                 const float m_new = grow ? top : m;
                 const float alpha = grow ? ex2((m - m_new) * c) : 1.f;
                 m = m_new;
                 l *= alpha;
-                if (j > first) {
-#pragma unroll
-                    for (int k = 0; k < DP; k += 32) {
-                        float o[32];
-                        tmem_ld32_nowait(t_o + k, o);
+                if (done) {
+                    // the half-step before has been added to O
+                    if (!(ok = wait(pv_done(i, h ^ 1), (done - 1) >> 1 & 1u))) break;
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int k = 0; k < DP; k += 16) {
+                        float o[16];
+                        tmem_ld16(t_o + k, o);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] *= alpha;
-                        tmem_st32(t_o + k, reinterpret_cast<uint32_t *>(o));
+                        for (int e = 0; e < 16; ++e) o[e] *= alpha;
+                        tmem_st16(t_o + k, reinterpret_cast<uint32_t *>(o));
                     }
                 }
             }
-            const float off = m == -INFINITY ? 0.f : -m * c;
-            const uint64_t c2 = f2splat(c), off2 = f2splat(off);
             uint64_t sum2[2] = {0, 0};
-#pragma unroll
-            for (int k0 = 0; k0 < 128; k0 += 64) {
-                uint32_t pk[32];
-#pragma unroll
-                for (int k = 0; k < 64; k += 2) {
-                    const uint64_t x = f2fma(f2pack(__float_as_uint(s[k0 + k]), __float_as_uint(s[k0 + k + 1])), c2, off2);
-                    float e0, e1;
-                    f2unpack(x, e0, e1);
-                    e0 = ex2(e0);
-                    e1 = ex2(e1);
-                    pk[k / 2] = pack16<BF16>(e0, e1);
-                    sum2[(k / 2) & 1] = f2add(sum2[(k / 2) & 1], f2pack(__float_as_uint(e0), __float_as_uint(e1)));
-                }
-                tmem_st32(t_s + k0 / 2, pk);
-            }
+            uint32_t pk[32];
+            exps<BF16, 64>(s, f2splat(c), f2splat(m == -INFINITY ? 0.f : -m * c), pk, sum2);
+            tmem_st32(t_s + h * 64, pk);
             float s0, s1, s2, s3;
             f2unpack(sum2[0], s0, s1);
             f2unpack(sum2[1], s2, s3);
             l += (s0 + s1) + (s2 + s3);
             tmem_wait_st();
             tc_fence_before();
-            bar_arrive(p_full(i));
+            warp_arrive(p_full(i, h));
         }
         // ---- results of the row
         const bool any = first < last;
-        if (any && ok) ok = __all_sync(0xffffffffu, wait(o_full(i), 0, abort_flag, p.status));
+        if (any && ok) ok = wait(pv_done(i, (last - 1) & 1), (uint32_t)(last - 1 - first) >> 1 & 1u);
+        if (!ok && lane == 0) atomicOr(p.status, kStatusTimeout);
         tc_fence_after();
         const uint64_t token = (uint64_t)w.rq.first + row / (int32_t)p.group;
         const uint32_t head = w.h * p.group + row % (int32_t)p.group;
@@ -550,7 +606,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             // ---- the share that finishes last adds them all, in order
             __threadfence();
             softmax_sync();
-            if (threadIdx.x == 0) {
+            if (tid == 0) {
                 const uint32_t before = atomicAdd(p.counters + w.group_index, 1u);
                 *last_flag = before + 1 == w.n_split;
                 if (before + 1 == w.n_split) p.counters[w.group_index] = 0u;
@@ -559,8 +615,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (*last_flag && valid) {
             __threadfence();
             const uint64_t part0 = (uint64_t)w.group_index * p.splits;
-            const float2 *ml = reinterpret_cast<const float2 *>(p.ws) + part0 * kChunkRows + threadIdx.x;
-            const float *po = p.ws + p.ws_ml + part0 * DP * kChunkRows + threadIdx.x;
+            const float2 *ml = reinterpret_cast<const float2 *>(p.ws) + part0 * kChunkRows + tid;
+            const float *po = p.ws + p.ws_ml + part0 * DP * kChunkRows + tid;
             float mm = -INFINITY, ll = 0.f;
             for (uint32_t s = 0; s < w.n_split; ++s) mm = fmaxf(mm, __ldcg(ml + (uint64_t)s * kChunkRows).x);
             const float base = mm == -INFINITY ? 0.f : mm;
@@ -591,7 +647,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     tc_fence_before();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == 8) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::tmem_cols));
     }
@@ -604,11 +660,6 @@ cudaError_t launch_inst(const CUtensorMap &km, const CUtensorMap &vm, const Attn
     static DeviceCache cache;
     int unused = 0;
     cudaError_t e = per_device(cache, unused, [&](int &) {
-        // the registers that the warpgroups share out must have been launched
-        cudaFuncAttributes attr{};
-        const cudaError_t q = cudaFuncGetAttributes(&attr, kernel);
-        if (q != cudaSuccess) return q;
-        if (attr.numRegs != kLaunchRegs) return cudaErrorInvalidKernelImage;
         return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::bytes);
     });
     if (e != cudaSuccess) return e;
