@@ -58,14 +58,16 @@ __device__ __forceinline__ Request load_request(const BatchView &bt, uint32_t pa
 
 // Page number of entry j of request b's row (j < table_width).  A number
 // outside the cache sets TC_STATUS_GEOMETRY and gives -1.
-__device__ __forceinline__ int32_t load_page(const BatchView &bt, uint32_t n_pages, uint32_t b, uint32_t j,
-                                             uint32_t *status) {
-    const int32_t p = bt.page_table[(uint64_t)b * bt.ld_table + j];
+__device__ __forceinline__ int32_t check_page(int32_t p, uint32_t n_pages, uint32_t *status) {
     if (p < 0 || (uint32_t)p >= n_pages) {
         atomicOr(status, kStatusGeometry);
         return -1;
     }
     return p;
+}
+__device__ __forceinline__ int32_t load_page(const BatchView &bt, uint32_t n_pages, uint32_t b, uint32_t j,
+                                             uint32_t *status) {
+    return check_page(bt.page_table[(uint64_t)b * bt.ld_table + j], n_pages, status);
 }
 
 // How many of the requests 1 .. n satisfy `before` (true for a prefix of

@@ -34,21 +34,25 @@ namespace {
 constexpr int kKeys = 16;        // keys of a warp's step
 constexpr int kWarps = 4;
 constexpr uint32_t kMaxChunk = 1024;
-constexpr uint64_t kFewRows = 16;   // rows of a request up to which this file's kernel is used
 
-template <int DP>
+// Rows of a CTA: MT mma tiles of 16.
+template <int DP, int MT>
 struct FewLayout {
     static constexpr int halves = DP / 64;
+    static constexpr int rows = 16 * MT;
     static constexpr uint32_t kv_bytes = kKeys * DP * 2;       // K of a step; V follows
     static constexpr uint32_t stage = 2 * kv_bytes;
-    static constexpr int stages = DP == 64 ? 6 : 3;
+    // 64 KB of rings: three CTAs per SM.  (Three stages and two CTAs kept as
+    // much in flight but took 265 us, not 245, for 1.5 GB of cache.)
+    static constexpr int stages = DP == 64 ? 4 : 2;
     static constexpr uint32_t ring = stages * stage;           // per warp
     static constexpr uint32_t bar_off = kWarps * ring;
     static constexpr uint32_t page_off = bar_off + kWarps * stages * 8;
-    static constexpr uint32_t ml_off = page_off + kMaxChunk / 8 * 4;    // [warp][16 rows][m, l]
-    static constexpr uint32_t misc_off = ml_off + kWarps * 16 * 8;
+    static constexpr uint32_t ml_off = page_off + (kMaxChunk / 8 + 2) * 4;   // [warp][row][m, l]
+    static constexpr uint32_t misc_off = ml_off + kWarps * rows * 8;
     static constexpr uint32_t bytes = misc_off + 16 + 1024;
-    static_assert(kWarps * ring >= kWarps * 16 * DP * 4, "the join reuses the rings");
+    static_assert(kWarps * ring >= kWarps * rows * DP * 4, "the join reuses the rings");
+    static constexpr uint32_t max_shares = kWarps * ring / (rows * 8);   // whose statistics fit there too
 };
 
 template <bool BF16>
@@ -77,29 +81,43 @@ __device__ __forceinline__ void ldsm4(uint32_t (&v)[4], uint32_t addr) {
 }
 
 // Two neighbouring 16-bit elements of q (pairs: 4-byte aligned) as one word.
-__device__ __forceinline__ uint32_t load_pair(const uint16_t *p, bool pairs, bool second) {
-    if (pairs) return *reinterpret_cast<const uint32_t *>(p);
-    return (uint32_t)p[0] | (second ? (uint32_t)p[1] << 16 : 0u);
+__device__ __forceinline__ uint32_t load_pair(const uint16_t *p, bool pairs) {
+    return pairs ? *reinterpret_cast<const uint32_t *>(p) : (uint32_t)p[0] | (uint32_t)p[1] << 16;
 }
 
-template <int DP, bool BF16>
+template <int DP, int MT, bool BF16>
 __global__ void __launch_bounds__(kWarps * 32)
     few_rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                     const __grid_constant__ AttnParams p) {
-    using L = FewLayout<DP>;
+    using L = FewLayout<DP, MT>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t split = blockIdx.x, h = blockIdx.y, b = blockIdx.z / p.row_tiles, rt = blockIdx.z % p.row_tiles;
     volatile uint32_t *abort_flag = reinterpret_cast<uint32_t *>(smem + L::misc_off);
     uint32_t *last_flag = reinterpret_cast<uint32_t *>(smem + L::misc_off) + 1;
+    const uint32_t bars = su32(smem + L::bar_off) + warp * L::stages * 8;
+    if (threadIdx.x < 2)
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(threadIdx.x ? &vmap : &kmap)) : "memory");
+    if (threadIdx.x == 0) *abort_flag = 0u;
+    if (lane == 0)
+        for (int i = 0; i < L::stages; ++i) bar_init(bars + 8 * i, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
 
+    // The entry of the page list that this thread will want if the first key
+    // is 0 (no window) travels with the request's values.
+    uint32_t guess = (split * p.chunk >> p.page_shift) + threadIdx.x;
+    int32_t guessed = -1;
+    if (guess < p.batch.table_width && threadIdx.x <= p.chunk >> p.page_shift)
+        guessed = p.batch.page_table[(uint64_t)b * p.batch.ld_table + guess];
+    else
+        guess = ~0u;
     const Request rq = load_request(p.batch, p.page_shift, b, p.status);
-    const int32_t n_rows = rq.n_new * (int32_t)p.group, row0 = (int32_t)rt * 16;
+    const int32_t n_rows = rq.n_new * (int32_t)p.group, row0 = (int32_t)rt * L::rows;
     if (row0 >= n_rows) return;
     // keys that any row of the tile sees, and this CTA's share
     const int32_t place0 = rq.length - rq.n_new;
-    const int32_t tok0 = row0 / (int32_t)p.group, tok1 = (min(row0 + 16, n_rows) - 1) / (int32_t)p.group;
+    const int32_t tok0 = row0 / (int32_t)p.group, tok1 = (min(row0 + L::rows, n_rows) - 1) / (int32_t)p.group;
     int32_t lo, hi, unused;
     visible(place0 + tok0, rq.length, p.causal, p.window, lo, unused);
     visible(place0 + tok1, rq.length, p.causal, p.window, unused, hi);
@@ -112,71 +130,67 @@ __global__ void __launch_bounds__(kWarps * 32)
     }
     const int32_t begin = base + (int32_t)(split * p.chunk), end = hi > lo ? min(hi, begin + (int32_t)p.chunk) : begin;
 
-    // ---- page numbers of the chunk, barriers
+    // ---- page numbers of the chunk
     int32_t *pages = reinterpret_cast<int32_t *>(smem + L::page_off);
-    const uint32_t bars = su32(smem + L::bar_off) + warp * L::stages * 8;
     if (end > begin) {
         const uint32_t j0 = (uint32_t)begin >> p.page_shift, j1 = (uint32_t)(end - 1) >> p.page_shift;
         for (uint32_t j = j0 + threadIdx.x; j <= j1; j += kWarps * 32)
-            pages[j - j0] = max(load_page(p.batch, p.n_pages, b, j, p.status), 0);
+            pages[j - j0] = j == guess ? check_page(guessed, p.n_pages, p.status)
+                                       : load_page(p.batch, p.n_pages, b, j, p.status);
     }
-    if (threadIdx.x == 0) *abort_flag = 0u;
-    if (lane == 0)
-        for (int i = 0; i < L::stages; ++i) bar_init(bars + 8 * i, 1);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+
     __syncthreads();
 
     const uint32_t ring = su32(smem) + warp * L::ring;
     const int32_t steps = (end - begin + kKeys - 1) / kKeys;
     const uint32_t box = min((uint32_t)kKeys, 1u << p.page_shift);   // tokens of a TMA box
-    // Loads of the warp's step i (16 keys from `key`): boxes of both halves of
-    // each page piece that begins before the chunk's end.
+    // Loads of the warp's step i (16 keys from `key`), a lane for each box: K or
+    // V, half, and page piece, of the pieces that begin before the chunk's end.
+    const uint32_t box_half = lane / 2 % L::halves, box_piece = lane / 2 / L::halves;
     auto issue = [&](int32_t i, uint32_t st) {
         const int32_t key = begin + i * kKeys;
         const uint32_t pieces = min((uint32_t)kKeys / box, (uint32_t)(end - key + (int32_t)box - 1) / box);
-        const uint32_t bar = bars + 8 * st, dst = ring + st * L::stage;
-        bar_expect_tx(bar, pieces * box * DP * 4);
-        for (uint32_t c = 0; c < pieces; ++c) {
-            const uint32_t pos = (uint32_t)key + c * box;
-            const int page = pages[(pos >> p.page_shift) - ((uint32_t)begin >> p.page_shift)];
-            const int token = (int)(pos & ((1u << p.page_shift) - 1));
-#pragma unroll
-            for (int hf = 0; hf < L::halves; ++hf) {
-                tma_load_4d(dst + hf * (kKeys * 128) + c * box * 128, &kmap, bar, hf * 64, token, (int)h, page);
-                tma_load_4d(dst + L::kv_bytes + hf * (kKeys * 128) + c * box * 128, &vmap, bar, hf * 64, token, (int)h,
-                            page);
-            }
+        const uint32_t bar = bars + 8 * st;
+        if (lane == 0) bar_expect_tx(bar, pieces * box * DP * 4);
+        __syncwarp();
+        if (box_piece < pieces) {
+            const uint32_t pos = (uint32_t)key + box_piece * box;
+            const int page = max(pages[(pos >> p.page_shift) - ((uint32_t)begin >> p.page_shift)], 0);
+            tma_load_4d(ring + st * L::stage + (lane & 1) * L::kv_bytes + box_half * (kKeys * 128) + box_piece * box * 128,
+                        lane & 1 ? &vmap : &kmap, bar, (int)box_half * 64, (int)(pos & ((1u << p.page_shift) - 1)),
+                        (int)h, page);
         }
     };
-    if (lane == 0)
-        for (int32_t s = 0; s < L::stages; ++s)
-            if ((int32_t)warp + s * kWarps < steps) issue((int32_t)warp + s * kWarps, (uint32_t)s);
-    __syncwarp();
+    for (int32_t s = 0; s < L::stages; ++s)
+        if ((int32_t)warp + s * kWarps < steps) issue((int32_t)warp + s * kWarps, (uint32_t)s);
 
     // ---- queries in registers (row-major A fragments)
     const uint32_t g = lane / 4, t4 = lane % 4;
-    uint32_t qf[DP / 16][4];
-    int32_t row_lo[2], row_hi[2];
+    uint32_t qf[MT][DP / 16][4];
+    int32_t row_lo[MT][2], row_hi[MT][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int32_t r = row0 + (int32_t)g + 8 * i;
-        const bool on = r < n_rows;
-        const int32_t tok = on ? r / (int32_t)p.group : 0;
-        visible(place0 + tok, rq.length, p.causal, p.window, row_lo[i], row_hi[i]);
-        if (!on) row_hi[i] = 0;
-        const uint16_t *q = p.q + (uint64_t)(rq.first + tok) * p.ld_q_token +
-                            (uint64_t)(h * p.group + (on ? r % (int32_t)p.group : 0)) * p.ld_q_head;
+    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks)
+        for (int i = 0; i < 2; ++i) {
+            const int32_t r = row0 + mt * 16 + (int32_t)g + 8 * i;
+            const bool on = r < n_rows;
+            const int32_t tok = on ? r / (int32_t)p.group : 0;
+            visible(place0 + tok, rq.length, p.causal, p.window, row_lo[mt][i], row_hi[mt][i]);
+            if (!on) row_hi[mt][i] = 0;
+            const uint16_t *q = p.q + (uint64_t)(rq.first + tok) * p.ld_q_token +
+                                (uint64_t)(h * p.group + (on ? r % (int32_t)p.group : 0)) * p.ld_q_head;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const uint32_t d = ks * 16 + j * 8 + t4 * 2;
-                qf[ks][i + 2 * j] = on && d < p.head_dim ? load_pair(q + d, p.q_pairs, true) : 0u;
-            }
-    }
-
-    float o[DP / 8][4] = {};
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {};
+            for (int ks = 0; ks < DP / 16; ++ks)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const uint32_t d = ks * 16 + j * 8 + t4 * 2;
+                    qf[mt][ks][i + 2 * j] = on && d < p.head_dim ? load_pair(q + d, p.q_pairs) : 0u;
+                }
+        }
+    float o[MT][DP / 8][4] = {};
+    float m[MT][2], l[MT][2];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) m[mt][0] = m[mt][1] = -INFINITY, l[mt][0] = l[mt][1] = 0.f;
     uint32_t st = 0, ph = 0;
     for (int32_t i = (int32_t)warp; i < steps; i += kWarps) {
         const int32_t key = begin + i * kKeys;
@@ -197,7 +211,7 @@ __global__ void __launch_bounds__(kWarps * 32)
             fence_proxy_async();   // before a later copy into the stage
             __syncwarp();
         }
-        float s[2][4] = {};
+        float s[MT][2][4] = {};
         const uint32_t lr = lane & 7, li = lane >> 3;
         {
             const uint32_t kr = (li >> 1) * 8 + lr;
@@ -206,54 +220,60 @@ __global__ void __launch_bounds__(kWarps * 32)
                 const uint32_t x = ks * 2 + (li & 1);
                 uint32_t bf[4];
                 ldsm4<false>(bf, ks_addr + (x >> 3) * (kKeys * 128) + kr * 128 + (((x & 7) ^ lr) << 4));
-                mma16816<BF16>(s[0], qf[ks], bf[0], bf[1]);
-                mma16816<BF16>(s[1], qf[ks], bf[2], bf[3]);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    mma16816<BF16>(s[mt][0], qf[mt][ks], bf[0], bf[1]);
+                    mma16816<BF16>(s[mt][1], qf[mt][ks], bf[2], bf[3]);
+                }
             }
         }
-        // scale to powers of two, mask, running maximum
-        float mx[2] = {m[0], m[1]};
+        uint32_t pf[MT][4];
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int32_t j = key + n * 8 + (int32_t)t4 * 2 + (c & 1);
-                const bool seen = j >= row_lo[c >> 1] && j < row_hi[c >> 1];
-                s[n][c] = seen ? s[n][c] * p.scale_log2 : -INFINITY;
-                mx[c >> 1] = fmaxf(mx[c >> 1], s[n][c]);
-            }
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-            mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-        }
-        if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
-            float al[2];
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                al[r] = mx[r] > m[r] ? exp2f(m[r] - mx[r]) : 1.f;
-                l[r] *= al[r];
-                m[r] = mx[r];
-            }
-#pragma unroll
-            for (int n = 0; n < DP / 8; ++n) {
-                o[n][0] *= al[0];
-                o[n][1] *= al[0];
-                o[n][2] *= al[1];
-                o[n][3] *= al[1];
-            }
-        }
-        uint32_t pf[4];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const float mm = m[r] == -INFINITY ? 0.f : m[r];
-            float e[4];
+        for (int mt = 0; mt < MT; ++mt) {
+            // scale to powers of two, mask, running maximum
+            float mx[2] = {m[mt][0], m[mt][1]};
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
-                for (int c = 0; c < 2; ++c) e[n * 2 + c] = exp2f(s[n][r * 2 + c] - mm);
-            l[r] += (e[0] + e[1]) + (e[2] + e[3]);
-            pf[r] = pack16<BF16>(e[0], e[1]);
-            pf[r + 2] = pack16<BF16>(e[2], e[3]);
+                for (int c = 0; c < 4; ++c) {
+                    const int32_t j = key + n * 8 + (int32_t)t4 * 2 + (c & 1);
+                    const bool seen = j >= row_lo[mt][c >> 1] && j < row_hi[mt][c >> 1];
+                    s[mt][n][c] = seen ? s[mt][n][c] * p.scale_log2 : -INFINITY;
+                    mx[c >> 1] = fmaxf(mx[c >> 1], s[mt][n][c]);
+                }
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+                mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+            }
+            if (__any_sync(0xffffffffu, mx[0] > m[mt][0] || mx[1] > m[mt][1])) {
+                float al[2];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    al[r] = mx[r] > m[mt][r] ? exp2f(m[mt][r] - mx[r]) : 1.f;
+                    l[mt][r] *= al[r];
+                    m[mt][r] = mx[r];
+                }
+#pragma unroll
+                for (int n = 0; n < DP / 8; ++n) {
+                    o[mt][n][0] *= al[0];
+                    o[mt][n][1] *= al[0];
+                    o[mt][n][2] *= al[1];
+                    o[mt][n][3] *= al[1];
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const float mm = m[mt][r] == -INFINITY ? 0.f : m[mt][r];
+                float e[4];
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) e[n * 2 + c] = exp2f(s[mt][n][r * 2 + c] - mm);
+                l[mt][r] += (e[0] + e[1]) + (e[2] + e[3]);
+                pf[mt][r] = pack16<BF16>(e[0], e[1]);
+                pf[mt][r + 2] = pack16<BF16>(e[2], e[3]);
+            }
         }
         {
             const uint32_t kr = (li & 1) * 8 + lr;
@@ -262,12 +282,15 @@ __global__ void __launch_bounds__(kWarps * 32)
                 const uint32_t x = n * 2 + (li >> 1);
                 uint32_t bf[4];
                 ldsm4<true>(bf, vs_addr + (x >> 3) * (kKeys * 128) + kr * 128 + (((x & 7) ^ lr) << 4));
-                mma16816<BF16>(o[2 * n], pf, bf[0], bf[1]);
-                mma16816<BF16>(o[2 * n + 1], pf, bf[2], bf[3]);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    mma16816<BF16>(o[mt][2 * n], pf[mt], bf[0], bf[1]);
+                    mma16816<BF16>(o[mt][2 * n + 1], pf[mt], bf[2], bf[3]);
+                }
             }
         }
         __syncwarp();   // every lane has read the stage
-        if (lane == 0 && i + L::stages * kWarps < steps) issue(i + L::stages * kWarps, st);
+        if (i + L::stages * kWarps < steps) issue(i + L::stages * kWarps, st);
         if (++st == L::stages) { st = 0; ph ^= 1; }
     }
     if (*abort_flag) {   // every copy issued has landed before the memory is reused or the CTA exits
@@ -278,42 +301,42 @@ __global__ void __launch_bounds__(kWarps * 32)
     }
 
     // ---- join the warps
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-    }
     __syncthreads();   // the rings are free
-    float *ow = reinterpret_cast<float *>(smem) + warp * 16 * DP;
+    float *ow = reinterpret_cast<float *>(smem) + warp * L::rows * DP;
     float2 *ml = reinterpret_cast<float2 *>(smem + L::ml_off);
 #pragma unroll
-    for (int n = 0; n < DP / 8; ++n)
+    for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
-            *reinterpret_cast<float2 *>(ow + (g + 8 * r) * DP + ((n * 8 + t4 * 2) ^ ((g & 3) * 8))) =
-                make_float2(o[n][2 * r], o[n][2 * r + 1]);
-    if (t4 == 0) {
-        ml[warp * 16 + g] = make_float2(m[0], l[0]);
-        ml[warp * 16 + g + 8] = make_float2(m[1], l[1]);
+        for (int r = 0; r < 2; ++r) {
+            l[mt][r] += __shfl_xor_sync(0xffffffffu, l[mt][r], 1);
+            l[mt][r] += __shfl_xor_sync(0xffffffffu, l[mt][r], 2);
+            if (t4 == 0) ml[warp * L::rows + mt * 16 + g + 8 * r] = make_float2(m[mt][r], l[mt][r]);
+        }
+#pragma unroll
+        for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+                *reinterpret_cast<float2 *>(ow + (mt * 16 + g + 8 * r) * DP + ((n * 8 + t4 * 2) ^ ((g & 3) * 8))) =
+                    make_float2(o[mt][n][2 * r], o[mt][n][2 * r + 1]);
     }
     __syncthreads();
-    const uint32_t rows = (uint32_t)min(16, n_rows - row0);
+    const uint32_t rows = (uint32_t)min(L::rows, n_rows - row0);
     const uint32_t tile = blockIdx.z * p.n_kv + h;
     const float *oall = reinterpret_cast<const float *>(smem);
     constexpr uint32_t quads = DP / 4;
-    // thread -> rows (threadIdx.x / quads) + ..., elements 4 * (threadIdx.x % quads)
+    // element e: row e / quads, elements 4 (e % quads) ..
     for (uint32_t e = threadIdx.x; e < rows * quads; e += kWarps * 32) {
         const uint32_t r = e / quads, d = (e % quads) * 4;
         float mm = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, ml[w * 16 + r].x);
+        for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, ml[w * L::rows + r].x);
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         float ll = 0.f;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-            const float2 v = ml[w * 16 + r];
+            const float2 v = ml[w * L::rows + r];
             const float a = v.x == -INFINITY ? 0.f : exp2f(v.x - mm);
-            const float4 x = *reinterpret_cast<const float4 *>(oall + (w * 16 + r) * DP + (d ^ ((r & 3) * 8)));
+            const float4 x = *reinterpret_cast<const float4 *>(oall + (w * L::rows + r) * DP + (d ^ ((r & 3) * 8)));
             acc.x += a * x.x;
             acc.y += a * x.y;
             acc.z += a * x.z;
@@ -330,30 +353,93 @@ __global__ void __launch_bounds__(kWarps * 32)
     }
     if (n_split == 1) return;
 
-    // ---- the chunk that finishes last adds them all, in order
-    __threadfence();
+    // ---- the share that finishes last adds them all, in order
     __syncthreads();
     if (threadIdx.x == 0) {
+        __threadfence();
         const uint32_t before = atomicAdd(p.counters + tile, 1u);
         *last_flag = before + 1 == n_split;
         if (before + 1 == n_split) p.counters[tile] = 0u;
+        __threadfence();
     }
     __syncthreads();
     if (!*last_flag) return;
-    __threadfence();
-    for (uint32_t e = threadIdx.x; e < rows * quads; e += kWarps * 32) {
-        const uint32_t r = e / quads, d = (e % quads) * 4;
-        const float2 *mls = reinterpret_cast<const float2 *>(p.ws) + (uint64_t)tile * p.splits * p.ws_rows + r;
-        const float *os = p.ws + p.ws_ml + ((uint64_t)tile * p.splits * p.ws_rows + r) * DP + d;
+    const float2 *mls = reinterpret_cast<const float2 *>(p.ws) + (uint64_t)tile * p.splits * p.ws_rows;
+    const float *os = p.ws + p.ws_ml + (uint64_t)tile * p.splits * p.ws_rows * DP;
+    float2 *part = reinterpret_cast<float2 *>(smem);   // [share][row]: maximum, then weight; sum
+    if (n_split <= L::max_shares) {
+        // The shares' statistics first, a few threads per row, then the
+        // outputs: two rounds of loads in flight together, not one a share.
+        constexpr uint32_t lanes = kWarps * 32 / L::rows;   // threads per row
+        constexpr uint32_t ahead = 8;
+        float4 first[ahead];   // of this thread's first elements: they need no weight to travel
+        const uint32_t e0 = min(threadIdx.x, rows * quads - 1);
+#pragma unroll
+        for (uint32_t s = 0; s < ahead; ++s)
+            first[s] = __ldcg(reinterpret_cast<const float4 *>(
+                os + ((uint64_t)min(s, n_split - 1) * p.ws_rows + e0 / quads) * DP + (e0 % quads) * 4));
+        const uint32_t r = threadIdx.x / lanes, s0 = threadIdx.x % lanes;
         float mm = -INFINITY, ll = 0.f;
+        if (r < rows) {
+#pragma unroll 4
+            for (uint32_t s = s0; s < n_split; s += lanes) {
+                const float2 v = __ldcg(mls + (uint64_t)s * p.ws_rows + r);
+                part[s * L::rows + r] = v;
+                mm = fmaxf(mm, v.x);
+            }
+        }
+#pragma unroll
+        for (uint32_t d = lanes / 2; d > 0; d /= 2) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
+        if (r < rows) {
+            for (uint32_t s = s0; s < n_split; s += lanes) {
+                const float2 v = part[s * L::rows + r];
+                const float a = v.x == -INFINITY ? 0.f : exp2f(v.x - mm);
+                part[s * L::rows + r].x = a;
+                ll += a * v.y;
+            }
+        }
+#pragma unroll
+        for (uint32_t d = lanes / 2; d > 0; d /= 2) ll += __shfl_xor_sync(0xffffffffu, ll, d);
+        if (s0 == 0 && r < rows) ml[r] = make_float2(mm, ll);
+        __syncthreads();
+        for (uint32_t e = threadIdx.x; e < rows * quads; e += kWarps * 32) {
+            const uint32_t rr = e / quads, d = (e % quads) * 4;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            uint32_t s = 0;
+            if (e == threadIdx.x) {
+#pragma unroll
+                for (uint32_t f = 0; f < ahead; ++f) {
+                    const float a = f < n_split ? part[f * L::rows + rr].x : 0.f;
+                    acc.x += a * first[f].x;
+                    acc.y += a * first[f].y;
+                    acc.z += a * first[f].z;
+                    acc.w += a * first[f].w;
+                }
+                s = ahead;
+            }
 #pragma unroll 8
-        for (uint32_t s = 0; s < n_split; ++s) mm = fmaxf(mm, __ldcg(mls + (uint64_t)s * p.ws_rows).x);
+            for (; s < n_split; ++s) {
+                const float a = part[s * L::rows + rr].x;
+                const float4 x = __ldcg(reinterpret_cast<const float4 *>(os + ((uint64_t)s * p.ws_rows + rr) * DP + d));
+                acc.x += a * x.x;
+                acc.y += a * x.y;
+                acc.z += a * x.z;
+                acc.w += a * x.w;
+            }
+            store_row4<BF16>(p, rq, h, row0 + (int32_t)rr, d, acc, ml[rr].x, ml[rr].y);
+        }
+        return;
+    }
+    for (uint32_t e = threadIdx.x; e < rows * quads; e += kWarps * 32) {   // very many shares
+        const uint32_t r = e / quads, d = (e % quads) * 4;
+        float mm = -INFINITY, ll = 0.f;
+        for (uint32_t s = 0; s < n_split; ++s) mm = fmaxf(mm, __ldcg(mls + (uint64_t)s * p.ws_rows + r).x);
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
+#pragma unroll 4
         for (uint32_t s = 0; s < n_split; ++s) {
-            const float2 v = __ldcg(mls + (uint64_t)s * p.ws_rows);
+            const float2 v = __ldcg(mls + (uint64_t)s * p.ws_rows + r);
             const float a = v.x == -INFINITY ? 0.f : exp2f(v.x - mm);
-            const float4 x = __ldcg(reinterpret_cast<const float4 *>(os + (uint64_t)s * p.ws_rows * DP));
+            const float4 x = __ldcg(reinterpret_cast<const float4 *>(os + ((uint64_t)s * p.ws_rows + r) * DP + d));
             acc.x += a * x.x;
             acc.y += a * x.y;
             acc.z += a * x.z;
@@ -364,10 +450,10 @@ __global__ void __launch_bounds__(kWarps * 32)
     }
 }
 
-template <int DP, bool BF16>
+template <int DP, int MT, bool BF16>
 cudaError_t launch_few(const CUtensorMap &km, const CUtensorMap &vm, const AttnParams &p, dim3 grid, cudaStream_t s) {
-    using L = FewLayout<DP>;
-    auto kernel = few_rows_kernel<DP, BF16>;
+    using L = FewLayout<DP, MT>;
+    auto kernel = few_rows_kernel<DP, MT, BF16>;
     static DeviceCache cache;
     int unused = 0;
     cudaError_t e = per_device(cache, unused, [&](int &) {
@@ -378,10 +464,10 @@ cudaError_t launch_few(const CUtensorMap &km, const CUtensorMap &vm, const AttnP
     return cudaGetLastError();
 }
 
-template <int DP>
+template <int DP, int MT>
 cudaError_t launch_few_t(const CUtensorMap &km, const CUtensorMap &vm, const AttnParams &p, bool bf16, dim3 grid,
                          cudaStream_t s) {
-    return bf16 ? launch_few<DP, true>(km, vm, p, grid, s) : launch_few<DP, false>(km, vm, p, grid, s);
+    return bf16 ? launch_few<DP, MT, true>(km, vm, p, grid, s) : launch_few<DP, MT, false>(km, vm, p, grid, s);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -512,7 +598,11 @@ int attend(tc_cuda_ctx *ctx, const tc_paged_cache *cache, const tc_paged_batch *
     CurrentDevice guard(ctx->device);
 
     const uint64_t rows_most = group * p.batch.max_new;
-    if (rows_most > kFewRows && c.head_dim <= 128) {
+    // mma tiles of a CTA: all rows of a request in one CTA, so that K and V are
+    // read once, as far as the registers go.
+    const uint32_t dp = c.head_dim <= 64 ? 64 : c.head_dim <= 128 ? 128 : 256;
+    const uint32_t mt = rows_most <= 16 || dp == 256 ? 1 : rows_most <= 32 || dp == 128 ? 2 : 4;
+    if (rows_most > mt * 16 && c.head_dim <= 128) {
         const uint64_t rows = (uint64_t)p.batch.n_tokens * group;
         p.n_blocks = (uint32_t)(rows / kChunkRows + p.batch.n_seq);
         p.q_wide = !(reinterpret_cast<uintptr_t>(a->q) % 16) && !(a->ld_q_token % 8) && !(a->ld_q_head % 8);
@@ -539,7 +629,6 @@ int attend(tc_cuda_ctx *ctx, const tc_paged_cache *cache, const tc_paged_batch *
         p.chunk = (uint32_t)(share * kChunkKeys);
         p.splits = (uint32_t)((steps + share - 1) / share);
         if ((uint64_t)p.n_blocks * c.n_heads * p.splits > 0x7fffffffu) return fail("too many tokens or requests");
-        const uint64_t dp = c.head_dim <= 64 ? 64 : 128;
         if (p.splits > 1) {
             const uint64_t parts = (uint64_t)p.n_blocks * c.n_heads * p.splits * kChunkRows;
             p.ws_ml = parts * 2;
@@ -554,22 +643,28 @@ int attend(tc_cuda_ctx *ctx, const tc_paged_cache *cache, const tc_paged_batch *
         const cudaError_t e = launch_chunk(km, vm, p, bf16, s);
         return e == cudaSuccess ? ok() : cuda_fail("paged attention launch", e);
     }
-    p.row_tiles = (uint32_t)((rows_most + 15) / 16);
+    p.row_tiles = (uint32_t)((rows_most + 16 * mt - 1) / (16 * mt));
     const uint64_t units = (uint64_t)p.batch.n_seq * p.row_tiles;
     if (units > 65535) return fail("too many tokens or requests");
     span += kKeys;   // the first key is rounded down to a step
-    // Chunk of the cache per CTA: short enough that the largest possible work
-    // is about six CTAs for each one that fits on the GPU (two per SM), at
-    // least 128 keys, at most what the page list holds.
-    const uint64_t want = (uint64_t)ctx->sm_count * 2 * 6;
-    uint64_t chunk = (span * units * c.n_heads + want - 1) / want;
-    chunk = (chunk + 63) / 64 * 64;
-    if (chunk < 128) chunk = 128;
-    if (chunk > kMaxChunk) chunk = kMaxChunk;
+    // Chunk of the cache per CTA: the least of (rounds of CTAs over the GPU's
+    // places) x (a chunk's time + what a CTA costs besides) + the time to join
+    // the shares, all in keys: about 100 KB for a CTA's start and end (7 us
+    // against 15 GB/s a place), 8 keys a share.  23 requests of 2071 keys by 28
+    // rows: 3 shares, 17 us; with many short ones (11 shares) 41 us.
+    const uint64_t places = (uint64_t)ctx->sm_count * (mt == 1 ? 3 : 2), cta_keys = 100 * 1024 / (4 * dp);
+    uint64_t chunk = kMaxChunk, best = ~0ull;
+    for (uint64_t c = kMaxChunk; c >= 64; c -= 64) {
+        const uint64_t n = (span + c - 1) / c, rounds = (units * n * p.n_kv + places - 1) / places;
+        const uint64_t cost = rounds * (c + cta_keys) + 8 * n;
+        if (cost < best) {
+            best = cost;
+            chunk = c;
+        }
+    }
     p.chunk = (uint32_t)chunk;
     p.splits = (uint32_t)((span + chunk - 1) / chunk);
-    p.ws_rows = (uint32_t)(group * p.batch.max_new < 16 ? group * p.batch.max_new : 16);
-    const uint32_t dp = c.head_dim <= 64 ? 64 : c.head_dim <= 128 ? 128 : 256;
+    p.ws_rows = (uint32_t)std::min<uint64_t>(rows_most, 16 * mt);
     if (p.splits > 1) {
         const uint64_t parts = units * c.n_heads * p.splits * p.ws_rows;
         p.ws_ml = (parts * 2 + 3) / 4 * 4;
@@ -582,9 +677,15 @@ int attend(tc_cuda_ctx *ctx, const tc_paged_cache *cache, const tc_paged_batch *
     if (!encode_cache(&km, c.k, c, box, bf16) || !encode_cache(&vm, c.v, c, box, bf16))
         return fail("the cache cannot be described to TMA");
     const dim3 grid(p.splits, c.n_heads, (uint32_t)units);
-    cudaError_t e = dp == 64 ? launch_few_t<64>(km, vm, p, bf16, grid, s)
-                  : dp == 128 ? launch_few_t<128>(km, vm, p, bf16, grid, s)
-                              : launch_few_t<256>(km, vm, p, bf16, grid, s);
+    cudaError_t e;
+    if (dp == 64)
+        e = mt == 1   ? launch_few_t<64, 1>(km, vm, p, bf16, grid, s)
+            : mt == 2 ? launch_few_t<64, 2>(km, vm, p, bf16, grid, s)
+                      : launch_few_t<64, 4>(km, vm, p, bf16, grid, s);
+    else if (dp == 128)
+        e = mt == 1 ? launch_few_t<128, 1>(km, vm, p, bf16, grid, s) : launch_few_t<128, 2>(km, vm, p, bf16, grid, s);
+    else
+        e = launch_few_t<256, 1>(km, vm, p, bf16, grid, s);
     return e == cudaSuccess ? ok() : cuda_fail("paged attention launch", e);
 }
 
