@@ -551,7 +551,8 @@ int tc_cuda_kv_append(tc_cuda_ctx *ctx, const tc_paged_cache *cache, const tc_pa
  * infinity in a cached value that a row does not see may still reach rows of
  * the same request; past the request's length nothing is read into results.
  * Long caches are split over CTAs with partial results in the context's
- * workspace. */
+ * workspace, which grows on demand (outside stream captures: make the first
+ * call of the largest sizes before capturing). */
 typedef struct tc_attention {
     const void *q;
     void *out;

@@ -515,22 +515,27 @@ int cuda_fail(const char *what, cudaError_t e) {
 // Grows the context's split workspace; the counters start at zero and every
 // complete kernel leaves them so.
 int ensure_split(tc_cuda_ctx *ctx, size_t floats, size_t counters, cudaStream_t s) {
+    constexpr int room = sizeof(ctx->attn_outgrown) / sizeof(ctx->attn_outgrown[0]);
     if (floats > ctx->attn_ws_floats) {
-        if (ctx->attn_ws) cudaFree(ctx->attn_ws);
-        ctx->attn_ws = nullptr;
-        ctx->attn_ws_floats = 0;
-        const cudaError_t e = cudaMalloc(&ctx->attn_ws, floats * sizeof(float));
+        void *fresh = nullptr;
+        const size_t n = std::max(floats, 2 * ctx->attn_ws_floats);
+        if (ctx->attn_outgrown_n == room) return fail("the attention workspace has grown too often");
+        const cudaError_t e = cudaMalloc(&fresh, n * sizeof(float));
         if (e != cudaSuccess) return cuda_fail("attention workspace allocation", e);
-        ctx->attn_ws_floats = floats;
+        if (ctx->attn_ws) ctx->attn_outgrown[ctx->attn_outgrown_n++] = ctx->attn_ws;
+        ctx->attn_ws = static_cast<float *>(fresh);
+        ctx->attn_ws_floats = n;
     }
     if (counters > ctx->attn_counters_n) {
-        if (ctx->attn_counters) cudaFree(ctx->attn_counters);
-        ctx->attn_counters = nullptr;
-        ctx->attn_counters_n = 0;
-        cudaError_t e = cudaMalloc(&ctx->attn_counters, counters * sizeof(uint32_t));
-        if (e == cudaSuccess) e = cudaMemsetAsync(ctx->attn_counters, 0, counters * sizeof(uint32_t), s);
+        void *fresh = nullptr;
+        const size_t n = std::max(counters, 2 * ctx->attn_counters_n);
+        if (ctx->attn_outgrown_n == room) return fail("the attention workspace has grown too often");
+        cudaError_t e = cudaMalloc(&fresh, n * sizeof(uint32_t));
+        if (e == cudaSuccess && (e = cudaMemsetAsync(fresh, 0, n * sizeof(uint32_t), s)) != cudaSuccess) cudaFree(fresh);
         if (e != cudaSuccess) return cuda_fail("attention counter allocation", e);
-        ctx->attn_counters_n = counters;
+        if (ctx->attn_counters) ctx->attn_outgrown[ctx->attn_outgrown_n++] = ctx->attn_counters;
+        ctx->attn_counters = static_cast<uint32_t *>(fresh);
+        ctx->attn_counters_n = n;
     }
     return TC_CUDA_OK;
 }

@@ -136,6 +136,7 @@ void tc_cuda_free(tc_cuda_ctx *ctx) {
     if (ctx->split_ws) cudaFree(ctx->split_ws);
     if (ctx->attn_ws) cudaFree(ctx->attn_ws);
     if (ctx->attn_counters) cudaFree(ctx->attn_counters);
+    for (int i = 0; i < ctx->attn_outgrown_n; ++i) cudaFree(ctx->attn_outgrown[i]);
     for (int i = 0; i < 8; ++i) {
         if (ctx->push_stream[i]) cudaStreamDestroy(ctx->push_stream[i]);
         if (ctx->push_join[i]) cudaEventDestroy(ctx->push_join[i]);

@@ -33,11 +33,15 @@ struct tc_cuda_ctx {
     float *split_ws = nullptr;       // split-K partial products of the tensor-core GEMM
     size_t split_ws_floats = 0;
     // Split attention: partial outputs with their softmax statistics, and one
-    // arrival counter per group of splits, kept at 0 (both grow on demand).
+    // arrival counter per group of splits, kept at 0.  Both grow on demand, at
+    // least twofold, and the outgrown buffers live as long as the context:
+    // CUDA graphs captured before may still use them.
     float *attn_ws = nullptr;
     size_t attn_ws_floats = 0;
     uint32_t *attn_counters = nullptr;
     size_t attn_counters_n = 0;
+    void *attn_outgrown[64] = {};
+    int attn_outgrown_n = 0;
     // Streaming GGUF loader (tc_cuda_weight_load_gguf): two pinned host and
     // two device staging slots (grow-only), its stream and per-slot events.
     void *load_host[2] = {}, *load_dev[2] = {};
