@@ -480,29 +480,37 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int32_t first = i ? w.first[1] : w.first[0], last = i ? w.last[1] : w.last[0];
         // queries of both tiles: DP / 8 16-byte pieces a row, all 256 threads
         {
-            constexpr uint32_t per = DP / 8;
-            for (uint32_t c = tid; c < 256 * per; c += 256) {
-                const uint32_t r = c / per, x = c % per;
-                const int32_t row = w.row0 + (int32_t)r;
-                uint32_t v[4] = {};
-                if (row < w.n_rows && x * 8 < p.head_dim) {
-                    const uint16_t *q = p.q + (uint64_t)(w.rq.first + row / (int32_t)p.group) * p.ld_q_token +
-                                        (uint64_t)(w.h * p.group + row % (int32_t)p.group) * p.ld_q_head + x * 8;
+            // (eight loads in flight: one after the other they took 10 us)
+            constexpr uint32_t per = DP / 8, total = 256 * per / 256, batch = total < 8 ? total : 8;
+#pragma unroll 1
+            for (uint32_t c0 = 0; c0 < total; c0 += batch) {
+                uint32_t v[batch][4];
+#pragma unroll
+                for (uint32_t k = 0; k < batch; ++k) {
+                    const uint32_t c = tid + (c0 + k) * 256, r = c / per, x = c % per;
+                    const uint32_t row = (uint32_t)w.row0 + r, token = row / p.group;
+                    const uint16_t *q = p.q + ((uint64_t)w.rq.first + token) * p.ld_q_token +
+                                        (uint64_t)(w.h * p.group + row - token * p.group) * p.ld_q_head + x * 8;
+                    const bool on = row < (uint32_t)w.n_rows && x * 8 < p.head_dim;
                     if (p.q_wide) {
-                        const uint4 u = *reinterpret_cast<const uint4 *>(q);
-                        v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+                        const uint4 u = on ? *reinterpret_cast<const uint4 *>(q) : make_uint4(0u, 0u, 0u, 0u);
+                        v[k][0] = u.x; v[k][1] = u.y; v[k][2] = u.z; v[k][3] = u.w;
                     } else {
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) v[k] = (uint32_t)q[2 * k] | (uint32_t)q[2 * k + 1] << 16;
+                        for (int e = 0; e < 4; ++e)
+                            v[k][e] = on ? (uint32_t)q[2 * e] | (uint32_t)q[2 * e + 1] << 16 : 0u;
                     }
-                    if (p.negate_q)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) v[k] ^= 0x80008000u;
                 }
-                const uint32_t dst = su32(smem + L::q_off) + (r / 128) * L::tile_bytes + (x / 8) * L::half_bytes +
-                                     (r % 128) * 128 + (((x % 8) ^ (r % 8)) << 4);
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
-                             ::"r"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+#pragma unroll
+                for (uint32_t k = 0; k < batch; ++k) {
+                    const uint32_t c = tid + (c0 + k) * 256, r = c / per, x = c % per;
+                    const uint32_t dst = su32(smem + L::q_off) + (r / 128) * L::tile_bytes + (x / 8) * L::half_bytes +
+                                         (r % 128) * 128 + (((x % 8) ^ (r % 8)) << 4);
+                    const uint32_t sign = p.negate_q ? 0x80008000u : 0u;
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                                 ::"r"(dst), "r"(v[k][0] ^ sign), "r"(v[k][1] ^ sign), "r"(v[k][2] ^ sign),
+                                   "r"(v[k][3] ^ sign) : "memory");
+                }
             }
             fence_proxy_async();
             warp_arrive(q_full);
