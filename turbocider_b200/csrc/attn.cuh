@@ -28,32 +28,32 @@ struct CacheView {
     uint32_t n_pages, page_size, page_shift, n_heads, head_dim;
 };
 
-// One request of the step.  length < 0: nothing of it can be used (its
-// values in device memory are impossible).
+// One request of the step (no rows or length 0 where its values in device
+// memory are impossible).
 struct Request {
     int32_t first, n_new, length;   // first row of q, new tokens, cached tokens
 };
 
 #ifdef __CUDACC__
-// Request b with its values checked: rows inside q, a length that its row of
+// A request with its values checked: rows inside q, a length that its row of
 // the page table covers, nothing past the bounds the launch was sized by.
-__device__ __forceinline__ Request load_request(const BatchView &bt, uint32_t page_shift, uint32_t b,
-                                                uint32_t *status) {
-    Request r;
-    r.first = bt.new_offsets[b];
-    const int32_t end = bt.new_offsets[b + 1];
-    r.length = bt.lengths[b];
-    if (r.first < 0 || end < r.first || (uint32_t)end > bt.n_tokens) {
+__device__ __forceinline__ Request check_request(const BatchView &bt, uint32_t page_shift, int32_t first, int32_t end,
+                                                 int32_t length, uint32_t *status) {
+    Request r{first, end - first, length};
+    if (first < 0 || end < first || (uint32_t)end > bt.n_tokens) {
         atomicOr(status, kStatusGeometry);
         return Request{0, 0, 0};
     }
-    r.n_new = end - r.first;
-    if (r.length < 0 || (uint32_t)r.length > bt.max_length || (uint32_t)r.n_new > bt.max_new ||
-        ((uint64_t)bt.table_width << page_shift) < (uint64_t)r.length) {
+    if (length < 0 || (uint32_t)length > bt.max_length || (uint32_t)r.n_new > bt.max_new ||
+        ((uint64_t)bt.table_width << page_shift) < (uint64_t)length) {
         atomicOr(status, kStatusGeometry);
         r.length = 0;
     }
     return r;
+}
+__device__ __forceinline__ Request load_request(const BatchView &bt, uint32_t page_shift, uint32_t b,
+                                                uint32_t *status) {
+    return check_request(bt, page_shift, bt.new_offsets[b], bt.new_offsets[b + 1], bt.lengths[b], status);
 }
 
 // Page number of entry j of request b's row (j < table_width).  A number

@@ -206,10 +206,20 @@ __device__ __forceinline__ bool find_work(const AttnParams &p, Work &w) {
     auto first_block = [&](uint32_t b) {
         return (int64_t)p.batch.new_offsets[b] * p.group / kChunkRows + b;
     };
-    w.b = count_prefix(p.batch.n_seq - 1, [&](uint32_t b) { return first_block(b) <= (int64_t)blk; });
-    w.rq = load_request(p.batch, p.page_shift, w.b, p.status);
+    if (p.batch.n_seq <= 32) {   // all requests in one round of loads
+        const uint32_t lane = threadIdx.x & 31, mine = min(lane, p.batch.n_seq - 1);
+        const int32_t begin = p.batch.new_offsets[mine], end = p.batch.new_offsets[mine + 1];
+        const int32_t length = p.batch.lengths[mine];
+        const bool before = (int64_t)begin * p.group / kChunkRows + mine <= (int64_t)blk;
+        w.b = __popc(__ballot_sync(0xffffffffu, before && lane > 0 && lane < p.batch.n_seq));
+        w.rq = check_request(p.batch, p.page_shift, __shfl_sync(0xffffffffu, begin, w.b),
+                             __shfl_sync(0xffffffffu, end, w.b), __shfl_sync(0xffffffffu, length, w.b), p.status);
+    } else {
+        w.b = count_prefix(p.batch.n_seq - 1, [&](uint32_t b) { return first_block(b) <= (int64_t)blk; });
+        w.rq = load_request(p.batch, p.page_shift, w.b, p.status);
+    }
     w.n_rows = w.rq.n_new * (int32_t)p.group;
-    const int64_t row0 = ((int64_t)blk - first_block(w.b)) * kChunkRows;
+    const int64_t row0 = ((int64_t)blk - ((int64_t)w.rq.first * p.group / kChunkRows + w.b)) * kChunkRows;
     if (row0 < 0 || row0 >= w.n_rows) return false;
     w.row0 = (int32_t)row0;
     const int32_t place0 = w.rq.length - w.rq.n_new;
@@ -267,6 +277,14 @@ __device__ __forceinline__ void store_row32(const AttnParams &p, uint16_t *o, ui
     uint32_t w[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) w[i] = pack16<BF16>(v[2 * i] * inv, v[2 * i + 1] * inv);
+    if (p.out_wide >= 32 && c0 + 32 <= p.head_dim) {   // whole sectors
+#pragma unroll
+        for (int i = 0; i < 16; i += 8)
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                         ::"l"(o + c0 + 2 * i), "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]),
+                           "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7]) : "memory");
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const uint32_t d = c0 + 8 * i;

@@ -611,7 +611,8 @@ int attend(tc_cuda_ctx *ctx, const tc_paged_cache *cache, const tc_paged_batch *
         const uint64_t rows = (uint64_t)p.batch.n_tokens * group;
         p.n_blocks = (uint32_t)(rows / kChunkRows + p.batch.n_seq);
         p.q_wide = !(reinterpret_cast<uintptr_t>(a->q) % 16) && !(a->ld_q_token % 8) && !(a->ld_q_head % 8);
-        p.out_wide = !(reinterpret_cast<uintptr_t>(a->out) % 16) && !(a->ld_out_token % 8) && !(a->ld_out_head % 8);
+        const uint64_t out_bits = reinterpret_cast<uintptr_t>(a->out) | a->ld_out_token * 2 | a->ld_out_head * 2;
+        p.out_wide = out_bits % 32 == 0 ? 32 : out_bits % 16 == 0 ? 16 : 0;
         p.negate_q = p.scale_log2 < 0.f;
         p.scale_log2 = std::fabs(p.scale_log2);
         if (p.scale_log2 < 1e-30f) p.scale_log2 = 1e-30f;   // 0 * -inf would lose the mask
