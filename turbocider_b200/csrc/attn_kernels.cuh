@@ -24,8 +24,7 @@ struct AttnParams {
     uint64_t ws_ml;
     float *ws;
     uint32_t *counters;
-    bool q_pairs, out_quads;     // 4-byte loads of q / 8-byte stores of out are aligned
-    bool q_wide;                 // 16-byte loads of q are aligned
+    bool q_wide, out_quads;      // 16-byte loads of q / 8-byte stores of out are aligned
     uint32_t out_wide;           // bytes of an aligned store of out: 32, 16, or 0 for less
     uint32_t n_blocks;           // many rows: upper bound of the blocks of rows
     bool negate_q;               // many rows: scale_log2 is positive, the sign goes to q

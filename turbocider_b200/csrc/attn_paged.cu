@@ -31,7 +31,10 @@
 namespace tc {
 namespace {
 
-constexpr int kKeys = 16;        // keys of a warp's step
+// Keys of a warp's step: 32 for heads of up to 64, where 16 leave too little
+// between two waits (with the queries' loads, 23 requests by up to
+// 28 rows: 33 -> 20 us).
+constexpr int step_keys(int dp, int mt) { return dp == 64 && mt <= 2 ? 32 : 16; }
 constexpr int kWarps = 4;
 constexpr uint32_t kMaxChunk = 1024;
 
@@ -40,13 +43,15 @@ template <int DP, int MT>
 struct FewLayout {
     static constexpr int halves = DP / 64;
     static constexpr int rows = 16 * MT;
-    static constexpr uint32_t kv_bytes = kKeys * DP * 2;       // K of a step; V follows
+    static constexpr int keys = step_keys(DP, MT);
+    static constexpr uint32_t kv_bytes = keys * DP * 2;       // K of a step; V follows
     static constexpr uint32_t stage = 2 * kv_bytes;
     // 64 KB of rings: three CTAs per SM.  (Three stages and two CTAs kept as
     // much in flight but took 265 us, not 245, for 1.5 GB of cache.)
-    static constexpr int stages = DP == 64 ? 4 : 2;
+    static constexpr int stages = DP == 64 && keys == 16 ? 4 : 2;
     static constexpr uint32_t ring = stages * stage;           // per warp
-    static constexpr uint32_t bar_off = kWarps * ring;
+    static constexpr uint32_t q_off = kWarps * ring;           // queries: rows x DP, 16-byte pieces swizzled by row
+    static constexpr uint32_t bar_off = q_off + rows * DP * 2;
     static constexpr uint32_t page_off = bar_off + kWarps * stages * 8;
     static constexpr uint32_t ml_off = page_off + (kMaxChunk / 8 + 2) * 4;   // [warp][row][m, l]
     static constexpr uint32_t misc_off = ml_off + kWarps * rows * 8;
@@ -80,9 +85,87 @@ __device__ __forceinline__ void ldsm4(uint32_t (&v)[4], uint32_t addr) {
                      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr) : "memory");
 }
 
-// Two neighbouring 16-bit elements of q (pairs: 4-byte aligned) as one word.
-__device__ __forceinline__ uint32_t load_pair(const uint16_t *p, bool pairs) {
-    return pairs ? *reinterpret_cast<const uint32_t *>(p) : (uint32_t)p[0] | (uint32_t)p[1] << 16;
+// Adds the n_split shares of a tile in order and stores its rows.  R: rounds of
+// 128 threads x 4 elements that the rows take.
+template <int DP, int MT, bool BF16, int R>
+__device__ __forceinline__ void join_shares(const AttnParams &p, const Request &rq, uint32_t h, uint32_t tile,
+                                            int32_t row0, uint32_t rows, uint32_t n_split, float2 *part, float2 *ml) {
+    using L = FewLayout<DP, MT>;
+    constexpr uint32_t quads = DP / 4, threads = kWarps * 32;
+    const float2 *mls = reinterpret_cast<const float2 *>(p.ws) + (uint64_t)tile * p.splits * p.ws_rows;
+    const float *os = p.ws + p.ws_ml + (uint64_t)tile * p.splits * p.ws_rows * DP;
+    // `part` [share][row] (shared memory): maximum, then weight; sum.  The
+    // statistics first, a few threads per row; the first shares' outputs need no
+    // weight to travel and are on their way meanwhile.
+    constexpr uint32_t lanes = threads / L::rows, ahead = R == 1 ? 8 : 8 / R > 1 ? 8 / R : 1;
+    constexpr uint32_t together = R == 1 ? 16 : 16 / R > 1 ? 16 / R : 1;   // shares in flight after them
+    auto output = [&](uint32_t s, uint32_t k) {
+        const uint32_t e = min(threadIdx.x + k * threads, rows * quads - 1);
+        return __ldcg(reinterpret_cast<const float4 *>(
+            os + ((uint64_t)min(s, n_split - 1) * p.ws_rows + e / quads) * DP + (e % quads) * 4));
+    };
+    float4 first[ahead][R];
+#pragma unroll
+    for (uint32_t s = 0; s < ahead; ++s)
+#pragma unroll
+        for (uint32_t k = 0; k < R; ++k) first[s][k] = output(s, k);
+    const uint32_t r = threadIdx.x / lanes, s0 = threadIdx.x % lanes;
+    float mm = -INFINITY, ll = 0.f;
+    if (r < rows) {
+#pragma unroll 4
+        for (uint32_t s = s0; s < n_split; s += lanes) {
+            const float2 v = __ldcg(mls + (uint64_t)s * p.ws_rows + r);
+            part[s * L::rows + r] = v;
+            mm = fmaxf(mm, v.x);
+        }
+    }
+#pragma unroll
+    for (uint32_t d = lanes / 2; d > 0; d /= 2) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
+    if (r < rows) {
+        for (uint32_t s = s0; s < n_split; s += lanes) {
+            const float2 v = part[s * L::rows + r];
+            const float a = v.x == -INFINITY ? 0.f : exp2f(v.x - mm);
+            part[s * L::rows + r].x = a;
+            ll += a * v.y;
+        }
+    }
+#pragma unroll
+    for (uint32_t d = lanes / 2; d > 0; d /= 2) ll += __shfl_xor_sync(0xffffffffu, ll, d);
+    if (s0 == 0 && r < rows) ml[r] = make_float2(mm, ll);
+    __syncthreads();
+    float4 acc[R] = {};
+    auto add = [&](uint32_t s, uint32_t k, const float4 &x) {
+        const uint32_t e = min(threadIdx.x + k * threads, rows * quads - 1);
+        const float a = part[s * L::rows + e / quads].x;
+        acc[k].x += a * x.x;
+        acc[k].y += a * x.y;
+        acc[k].z += a * x.z;
+        acc[k].w += a * x.w;
+    };
+#pragma unroll
+    for (uint32_t s = 0; s < ahead; ++s)
+        if (s < n_split)
+#pragma unroll
+            for (uint32_t k = 0; k < R; ++k) add(s, k, first[s][k]);
+    for (uint32_t f = ahead; f < n_split; f += together) {
+        float4 x[together][R];
+#pragma unroll
+        for (uint32_t s = 0; s < together; ++s)
+#pragma unroll
+            for (uint32_t k = 0; k < R; ++k) x[s][k] = output(f + s, k);
+#pragma unroll
+        for (uint32_t s = 0; s < together; ++s)
+            if (f + s < n_split)
+#pragma unroll
+                for (uint32_t k = 0; k < R; ++k) add(f + s, k, x[s][k]);
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < R; ++k) {
+        const uint32_t e = threadIdx.x + k * threads;
+        if (e < rows * quads)
+            store_row4<BF16>(p, rq, h, row0 + (int32_t)(e / quads), (e % quads) * 4, acc[k], ml[e / quads].x,
+                             ml[e / quads].y);
+    }
 }
 
 template <int DP, int MT, bool BF16>
@@ -90,6 +173,7 @@ __global__ void __launch_bounds__(kWarps * 32)
     few_rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                     const __grid_constant__ AttnParams p) {
     using L = FewLayout<DP, MT>;
+    constexpr int kKeys = L::keys;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -164,29 +248,54 @@ __global__ void __launch_bounds__(kWarps * 32)
     for (int32_t s = 0; s < L::stages; ++s)
         if ((int32_t)warp + s * kWarps < steps) issue((int32_t)warp + s * kWarps, (uint32_t)s);
 
-    // ---- queries in registers (row-major A fragments)
+    // ---- queries through shared memory into row-major A fragments
     const uint32_t g = lane / 4, t4 = lane % 4;
     uint32_t qf[MT][DP / 16][4];
+    {
+        constexpr uint32_t per = DP / 8, rounds = L::rows * per / (kWarps * 32);
+        uint32_t v[rounds][4];
+#pragma unroll
+        for (uint32_t k = 0; k < rounds; ++k) {
+            const uint32_t c = threadIdx.x + k * kWarps * 32, x = c % per, row = (uint32_t)row0 + c / per;
+            const uint32_t tok = row / p.group;
+            const uint16_t *q = p.q + ((uint64_t)rq.first + tok) * p.ld_q_token +
+                                (uint64_t)(h * p.group + row - tok * p.group) * p.ld_q_head + x * 8;
+            const bool on = row < (uint32_t)n_rows && x * 8 < p.head_dim;
+            if (p.q_wide) {
+                const uint4 u = on ? *reinterpret_cast<const uint4 *>(q) : make_uint4(0u, 0u, 0u, 0u);
+                v[k][0] = u.x; v[k][1] = u.y; v[k][2] = u.z; v[k][3] = u.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[k][e] = on ? (uint32_t)q[2 * e] | (uint32_t)q[2 * e + 1] << 16 : 0u;
+            }
+        }
+        const uint32_t q_addr = su32(smem + L::q_off);
+#pragma unroll
+        for (uint32_t k = 0; k < rounds; ++k) {
+            const uint32_t c = threadIdx.x + k * kWarps * 32, x = c % per, r = c / per;
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                         ::"r"(q_addr + r * (DP * 2) + ((x ^ (r & 7)) << 4)), "r"(v[k][0]), "r"(v[k][1]), "r"(v[k][2]),
+                           "r"(v[k][3]) : "memory");
+        }
+        __syncthreads();
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int ks = 0; ks < DP / 16; ++ks) {
+                const uint32_t r = mt * 16 + (lane & 15), x = ks * 2 + (lane >> 4);
+                ldsm4<false>(qf[mt][ks], q_addr + r * (DP * 2) + ((x ^ (r & 7)) << 4));
+            }
+    }
     int32_t row_lo[MT][2], row_hi[MT][2];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int32_t r = row0 + mt * 16 + (int32_t)g + 8 * i;
-            const bool on = r < n_rows;
-            const int32_t tok = on ? r / (int32_t)p.group : 0;
-            visible(place0 + tok, rq.length, p.causal, p.window, row_lo[mt][i], row_hi[mt][i]);
-            if (!on) row_hi[mt][i] = 0;
-            const uint16_t *q = p.q + (uint64_t)(rq.first + tok) * p.ld_q_token +
-                                (uint64_t)(h * p.group + (on ? r % (int32_t)p.group : 0)) * p.ld_q_head;
-#pragma unroll
-            for (int ks = 0; ks < DP / 16; ++ks)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const uint32_t d = ks * 16 + j * 8 + t4 * 2;
-                    qf[mt][ks][i + 2 * j] = on && d < p.head_dim ? load_pair(q + d, p.q_pairs) : 0u;
-                }
+            visible(place0 + r / (int32_t)p.group, rq.length, p.causal, p.window, row_lo[mt][i], row_hi[mt][i]);
+            if (r >= n_rows) row_hi[mt][i] = 0;
         }
+
     float o[MT][DP / 8][4] = {};
     float m[MT][2], l[MT][2];
 #pragma unroll
@@ -211,29 +320,28 @@ __global__ void __launch_bounds__(kWarps * 32)
             fence_proxy_async();   // before a later copy into the stage
             __syncwarp();
         }
-        float s[MT][2][4] = {};
+        float s[MT][kKeys / 8][4] = {};
         const uint32_t lr = lane & 7, li = lane >> 3;
-        {
-            const uint32_t kr = (li >> 1) * 8 + lr;
 #pragma unroll
-            for (int ks = 0; ks < DP / 16; ++ks) {
-                const uint32_t x = ks * 2 + (li & 1);
+        for (int ks = 0; ks < DP / 16; ++ks)
+#pragma unroll
+            for (int kg = 0; kg < kKeys / 16; ++kg) {
+                const uint32_t x = ks * 2 + (li & 1), kr = kg * 16 + (li >> 1) * 8 + lr;
                 uint32_t bf[4];
                 ldsm4<false>(bf, ks_addr + (x >> 3) * (kKeys * 128) + kr * 128 + (((x & 7) ^ lr) << 4));
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
-                    mma16816<BF16>(s[mt][0], qf[mt][ks], bf[0], bf[1]);
-                    mma16816<BF16>(s[mt][1], qf[mt][ks], bf[2], bf[3]);
+                    mma16816<BF16>(s[mt][2 * kg], qf[mt][ks], bf[0], bf[1]);
+                    mma16816<BF16>(s[mt][2 * kg + 1], qf[mt][ks], bf[2], bf[3]);
                 }
             }
-        }
-        uint32_t pf[MT][4];
+        uint32_t pf[MT][kKeys / 16][4];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             // scale to powers of two, mask, running maximum
             float mx[2] = {m[mt][0], m[mt][1]};
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int n = 0; n < kKeys / 8; ++n)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     const int32_t j = key + n * 8 + (int32_t)t4 * 2 + (c & 1);
@@ -265,30 +373,32 @@ __global__ void __launch_bounds__(kWarps * 32)
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 const float mm = m[mt][r] == -INFINITY ? 0.f : m[mt][r];
-                float e[4];
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
+                for (int kg = 0; kg < kKeys / 16; ++kg) {
+                    float e[4];
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) e[n * 2 + c] = exp2f(s[mt][n][r * 2 + c] - mm);
-                l[mt][r] += (e[0] + e[1]) + (e[2] + e[3]);
-                pf[mt][r] = pack16<BF16>(e[0], e[1]);
-                pf[mt][r + 2] = pack16<BF16>(e[2], e[3]);
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) e[n * 2 + c] = exp2f(s[mt][2 * kg + n][r * 2 + c] - mm);
+                    l[mt][r] += (e[0] + e[1]) + (e[2] + e[3]);
+                    pf[mt][kg][r] = pack16<BF16>(e[0], e[1]);
+                    pf[mt][kg][r + 2] = pack16<BF16>(e[2], e[3]);
+                }
             }
         }
-        {
-            const uint32_t kr = (li & 1) * 8 + lr;
+#pragma unroll
+        for (int kg = 0; kg < kKeys / 16; ++kg)
 #pragma unroll
             for (int n = 0; n < DP / 16; ++n) {
-                const uint32_t x = n * 2 + (li >> 1);
+                const uint32_t x = n * 2 + (li >> 1), kr = kg * 16 + (li & 1) * 8 + lr;
                 uint32_t bf[4];
                 ldsm4<true>(bf, vs_addr + (x >> 3) * (kKeys * 128) + kr * 128 + (((x & 7) ^ lr) << 4));
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
-                    mma16816<BF16>(o[mt][2 * n], pf[mt], bf[0], bf[1]);
-                    mma16816<BF16>(o[mt][2 * n + 1], pf[mt], bf[2], bf[3]);
+                    mma16816<BF16>(o[mt][2 * n], pf[mt][kg], bf[0], bf[1]);
+                    mma16816<BF16>(o[mt][2 * n + 1], pf[mt][kg], bf[2], bf[3]);
                 }
             }
-        }
         __syncwarp();   // every lane has read the stage
         if (i + L::stages * kWarps < steps) issue(i + L::stages * kWarps, st);
         if (++st == L::stages) { st = 0; ph ^= 1; }
@@ -364,72 +474,17 @@ __global__ void __launch_bounds__(kWarps * 32)
     }
     __syncthreads();
     if (!*last_flag) return;
-    const float2 *mls = reinterpret_cast<const float2 *>(p.ws) + (uint64_t)tile * p.splits * p.ws_rows;
-    const float *os = p.ws + p.ws_ml + (uint64_t)tile * p.splits * p.ws_rows * DP;
-    float2 *part = reinterpret_cast<float2 *>(smem);   // [share][row]: maximum, then weight; sum
     if (n_split <= L::max_shares) {
-        // The shares' statistics first, a few threads per row, then the
-        // outputs: two rounds of loads in flight together, not one a share.
-        constexpr uint32_t lanes = kWarps * 32 / L::rows;   // threads per row
-        constexpr uint32_t ahead = 8;
-        float4 first[ahead];   // of this thread's first elements: they need no weight to travel
-        const uint32_t e0 = min(threadIdx.x, rows * quads - 1);
-#pragma unroll
-        for (uint32_t s = 0; s < ahead; ++s)
-            first[s] = __ldcg(reinterpret_cast<const float4 *>(
-                os + ((uint64_t)min(s, n_split - 1) * p.ws_rows + e0 / quads) * DP + (e0 % quads) * 4));
-        const uint32_t r = threadIdx.x / lanes, s0 = threadIdx.x % lanes;
-        float mm = -INFINITY, ll = 0.f;
-        if (r < rows) {
-#pragma unroll 4
-            for (uint32_t s = s0; s < n_split; s += lanes) {
-                const float2 v = __ldcg(mls + (uint64_t)s * p.ws_rows + r);
-                part[s * L::rows + r] = v;
-                mm = fmaxf(mm, v.x);
-            }
-        }
-#pragma unroll
-        for (uint32_t d = lanes / 2; d > 0; d /= 2) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
-        if (r < rows) {
-            for (uint32_t s = s0; s < n_split; s += lanes) {
-                const float2 v = part[s * L::rows + r];
-                const float a = v.x == -INFINITY ? 0.f : exp2f(v.x - mm);
-                part[s * L::rows + r].x = a;
-                ll += a * v.y;
-            }
-        }
-#pragma unroll
-        for (uint32_t d = lanes / 2; d > 0; d /= 2) ll += __shfl_xor_sync(0xffffffffu, ll, d);
-        if (s0 == 0 && r < rows) ml[r] = make_float2(mm, ll);
-        __syncthreads();
-        for (uint32_t e = threadIdx.x; e < rows * quads; e += kWarps * 32) {
-            const uint32_t rr = e / quads, d = (e % quads) * 4;
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-            uint32_t s = 0;
-            if (e == threadIdx.x) {
-#pragma unroll
-                for (uint32_t f = 0; f < ahead; ++f) {
-                    const float a = f < n_split ? part[f * L::rows + rr].x : 0.f;
-                    acc.x += a * first[f].x;
-                    acc.y += a * first[f].y;
-                    acc.z += a * first[f].z;
-                    acc.w += a * first[f].w;
-                }
-                s = ahead;
-            }
-#pragma unroll 8
-            for (; s < n_split; ++s) {
-                const float a = part[s * L::rows + rr].x;
-                const float4 x = __ldcg(reinterpret_cast<const float4 *>(os + ((uint64_t)s * p.ws_rows + rr) * DP + d));
-                acc.x += a * x.x;
-                acc.y += a * x.y;
-                acc.z += a * x.z;
-                acc.w += a * x.w;
-            }
-            store_row4<BF16>(p, rq, h, row0 + (int32_t)rr, d, acc, ml[rr].x, ml[rr].y);
-        }
+        constexpr int rounds = L::rows * quads / (kWarps * 32);
+        float2 *part = reinterpret_cast<float2 *>(smem);
+        if (rows * quads <= kWarps * 32)
+            join_shares<DP, MT, BF16, 1>(p, rq, h, tile, row0, rows, n_split, part, ml);
+        else
+            join_shares<DP, MT, BF16, rounds>(p, rq, h, tile, row0, rows, n_split, part, ml);
         return;
     }
+    const float2 *mls = reinterpret_cast<const float2 *>(p.ws) + (uint64_t)tile * p.splits * p.ws_rows;
+    const float *os = p.ws + p.ws_ml + (uint64_t)tile * p.splits * p.ws_rows * DP;
     for (uint32_t e = threadIdx.x; e < rows * quads; e += kWarps * 32) {   // very many shares
         const uint32_t r = e / quads, d = (e % quads) * 4;
         float mm = -INFINITY, ll = 0.f;
@@ -590,7 +645,7 @@ int attend(tc_cuda_ctx *ctx, const tc_paged_cache *cache, const tc_paged_batch *
     p.window = a->window > kMaxLength ? kMaxLength : a->window;
     p.scale_log2 = a->scale * 1.4426950408889634f;   // exp(x) = 2^(x log2 e)
     p.status = ctx->status;
-    p.q_pairs = !(reinterpret_cast<uintptr_t>(a->q) % 4) && !(a->ld_q_token % 2) && !(a->ld_q_head % 2);
+    p.q_wide = !(reinterpret_cast<uintptr_t>(a->q) % 16) && !(a->ld_q_token % 8) && !(a->ld_q_head % 8);
     p.out_quads = !(reinterpret_cast<uintptr_t>(a->out) % 8) && !(a->ld_out_token % 4) && !(a->ld_out_head % 4);
     const bool bf16 = cache->dtype == TC_DTYPE_BF16;
 
@@ -610,7 +665,6 @@ int attend(tc_cuda_ctx *ctx, const tc_paged_cache *cache, const tc_paged_batch *
     if (rows_most > mt * 16 && c.head_dim <= 128) {
         const uint64_t rows = (uint64_t)p.batch.n_tokens * group;
         p.n_blocks = (uint32_t)(rows / kChunkRows + p.batch.n_seq);
-        p.q_wide = !(reinterpret_cast<uintptr_t>(a->q) % 16) && !(a->ld_q_token % 8) && !(a->ld_q_head % 8);
         const uint64_t out_bits = reinterpret_cast<uintptr_t>(a->out) | a->ld_out_token * 2 | a->ld_out_head * 2;
         p.out_wide = out_bits % 32 == 0 ? 32 : out_bits % 16 == 0 ? 16 : 0;
         p.negate_q = p.scale_log2 < 0.f;
@@ -652,13 +706,14 @@ int attend(tc_cuda_ctx *ctx, const tc_paged_cache *cache, const tc_paged_batch *
     p.row_tiles = (uint32_t)((rows_most + 16 * mt - 1) / (16 * mt));
     const uint64_t units = (uint64_t)p.batch.n_seq * p.row_tiles;
     if (units > 65535) return fail("too many tokens or requests");
-    span += kKeys;   // the first key is rounded down to a step
+    const uint32_t keys = step_keys((int)dp, (int)mt);
+    span += keys;   // the first key is rounded down to a step
     // Chunk of the cache per CTA: the least of (rounds of CTAs over the GPU's
     // places) x (a chunk's time + what a CTA costs besides) + the time to join
     // the shares, all in keys: about 100 KB for a CTA's start and end (7 us
     // against 15 GB/s a place), 8 keys a share.  23 requests of 2071 keys by 28
     // rows: 3 shares, 17 us; with many short ones (11 shares) 41 us.
-    const uint64_t places = (uint64_t)ctx->sm_count * (mt == 1 ? 3 : 2), cta_keys = 100 * 1024 / (4 * dp);
+    const uint64_t places = (uint64_t)ctx->sm_count * (mt == 1 || (dp == 64 && mt == 2) ? 3 : 2), cta_keys = 100 * 1024 / (4 * dp);
     uint64_t chunk = kMaxChunk, best = ~0ull;
     for (uint64_t c = kMaxChunk; c >= 64; c -= 64) {
         const uint64_t n = (span + c - 1) / c, rounds = (units * n * p.n_kv + places - 1) / places;
@@ -679,7 +734,7 @@ int attend(tc_cuda_ctx *ctx, const tc_paged_cache *cache, const tc_paged_batch *
         p.counters = ctx->attn_counters;
     }
     CUtensorMap km, vm;
-    const uint32_t box = c.page_size < kKeys ? c.page_size : kKeys;
+    const uint32_t box = c.page_size < keys ? c.page_size : keys;
     if (!encode_cache(&km, c.k, c, box, bf16) || !encode_cache(&vm, c.v, c, box, bf16))
         return fail("the cache cannot be described to TMA");
     const dim3 grid(p.splits, c.n_heads, (uint32_t)units);
