@@ -345,6 +345,28 @@ __global__ void __launch_bounds__(kThreads, 1)
                      ::"r"(su32(tmem_slot)), "r"(L::tmem_cols));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
+    // Queries of both tiles, DP / 8 16-byte pieces a row over the 256 softmax
+    // threads, all in flight while the block sets up (one after the other they
+    // took 10 us of every CTA, in two rounds 3 us).
+    constexpr uint32_t q_per = DP / 8, q_rounds = q_per;
+    uint32_t qv[q_rounds][4];
+    if (warp < 8) {
+#pragma unroll
+        for (uint32_t k = 0; k < q_rounds; ++k) {
+            const uint32_t c = tid + k * 256, r = c / q_per, x = c % q_per;
+            const uint32_t row = (uint32_t)w.row0 + r, token = row / p.group;
+            const uint16_t *q = p.q + ((uint64_t)w.rq.first + token) * p.ld_q_token +
+                                (uint64_t)(w.h * p.group + row - token * p.group) * p.ld_q_head + x * 8;
+            const bool on = row < (uint32_t)w.n_rows && x * 8 < p.head_dim;
+            if (p.q_wide) {
+                const uint4 u = on ? *reinterpret_cast<const uint4 *>(q) : make_uint4(0u, 0u, 0u, 0u);
+                qv[k][0] = u.x; qv[k][1] = u.y; qv[k][2] = u.z; qv[k][3] = u.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) qv[k][e] = on ? (uint32_t)q[2 * e] | (uint32_t)q[2 * e + 1] << 16 : 0u;
+            }
+        }
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -496,39 +518,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         // ---------------------------------------------------- softmax
         const int i = warp / 4;
         const int32_t first = i ? w.first[1] : w.first[0], last = i ? w.last[1] : w.last[0];
-        // queries of both tiles: DP / 8 16-byte pieces a row, all 256 threads
+        // queries of both tiles into shared memory
         {
-            // (eight loads in flight: one after the other they took 10 us)
-            constexpr uint32_t per = DP / 8, total = 256 * per / 256, batch = total < 8 ? total : 8;
-#pragma unroll 1
-            for (uint32_t c0 = 0; c0 < total; c0 += batch) {
-                uint32_t v[batch][4];
 #pragma unroll
-                for (uint32_t k = 0; k < batch; ++k) {
-                    const uint32_t c = tid + (c0 + k) * 256, r = c / per, x = c % per;
-                    const uint32_t row = (uint32_t)w.row0 + r, token = row / p.group;
-                    const uint16_t *q = p.q + ((uint64_t)w.rq.first + token) * p.ld_q_token +
-                                        (uint64_t)(w.h * p.group + row - token * p.group) * p.ld_q_head + x * 8;
-                    const bool on = row < (uint32_t)w.n_rows && x * 8 < p.head_dim;
-                    if (p.q_wide) {
-                        const uint4 u = on ? *reinterpret_cast<const uint4 *>(q) : make_uint4(0u, 0u, 0u, 0u);
-                        v[k][0] = u.x; v[k][1] = u.y; v[k][2] = u.z; v[k][3] = u.w;
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            v[k][e] = on ? (uint32_t)q[2 * e] | (uint32_t)q[2 * e + 1] << 16 : 0u;
-                    }
-                }
-#pragma unroll
-                for (uint32_t k = 0; k < batch; ++k) {
-                    const uint32_t c = tid + (c0 + k) * 256, r = c / per, x = c % per;
-                    const uint32_t dst = su32(smem + L::q_off) + (r / 128) * L::tile_bytes + (x / 8) * L::half_bytes +
-                                         (r % 128) * 128 + (((x % 8) ^ (r % 8)) << 4);
-                    const uint32_t sign = p.negate_q ? 0x80008000u : 0u;
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
-                                 ::"r"(dst), "r"(v[k][0] ^ sign), "r"(v[k][1] ^ sign), "r"(v[k][2] ^ sign),
-                                   "r"(v[k][3] ^ sign) : "memory");
-                }
+            for (uint32_t k = 0; k < q_rounds; ++k) {
+                const uint32_t c = tid + k * 256, r = c / q_per, x = c % q_per;
+                const uint32_t dst = su32(smem + L::q_off) + (r / 128) * L::tile_bytes + (x / 8) * L::half_bytes +
+                                     (r % 128) * 128 + (((x % 8) ^ (r % 8)) << 4);
+                const uint32_t sign = p.negate_q ? 0x80008000u : 0u;
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                             ::"r"(dst), "r"(qv[k][0] ^ sign), "r"(qv[k][1] ^ sign), "r"(qv[k][2] ^ sign),
+                               "r"(qv[k][3] ^ sign) : "memory");
             }
             fence_proxy_async();
             warp_arrive(q_full);
@@ -610,7 +610,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (w.n_split > 1)
                 __stcg(reinterpret_cast<float2 *>(p.ws) + (uint64_t)w.part * kChunkRows + 128 * i + r,
                        make_float2(m * c, l));
-#pragma unroll 1
+#pragma unroll
             for (uint32_t k = 0; k < DP; k += 32) {
                 float o[32] = {};
                 if (any) {
