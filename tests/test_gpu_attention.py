@@ -70,6 +70,21 @@ def test_sizes_around_the_tiles(ctx, new, length, hq, hk, dim):
     attend(ctx, [(new, length), (max(new - 1, 1), length - 1)], 16, hq, hk, dim, BF, seed=new)
 
 
+@pytest.mark.parametrize("page", [512, 4096])
+@pytest.mark.parametrize("lens", [[(1, 1300), (1, 90)], [(9, 700), (1, 1)], [(200, 1300), (90, 90)]])
+def test_pages_larger_than_a_step(ctx, page, lens):
+    attend(ctx, lens, page, 4, 2, 128, BF, seed=page)
+
+
+@pytest.mark.parametrize("window", [0, 50])
+@pytest.mark.parametrize("new", [1, 6, 90])
+def test_many_requests(ctx, new, window):
+    """More requests than a warp looks up at once, of all sizes, empty ones
+    among them."""
+    lens = [((i * 7) % (new + 1), (i * 7) % (new + 1) + (i * 13) % 200) for i in range(71)] + [(0, 0), (new, 0), (0, 5)]
+    attend(ctx, lens, 16, 6, 2, 64, BF, seed=new, window=window)
+
+
 def test_rows_that_see_nothing_give_zeros(ctx):
     # more new tokens than cached ones: the first sit before the cache's start
     y, lse = attend(ctx, [(1, 0), (4, 0), (200, 0), (2, 30)], 16, 4, 2, 128, BF, seed=3)

@@ -7,6 +7,7 @@
 #include <cuda_fp16.h>
 
 #include <cstdint>
+#include <string>
 
 #include "../../include/turbocider_cuda.h"
 #include "tc_internal.h"
@@ -94,7 +95,34 @@ __device__ __forceinline__ void visible(int32_t p, int32_t length, int causal, i
 }
 #endif
 
-// Host-side checks shared by the entry points; nullptr: fine.
+// ---- host side of the entry points
+inline int fail(const char *reason) {
+    set_last_error(reason);
+    return TC_CUDA_FAIL;
+}
+inline int ok() {
+    set_last_error("");
+    return TC_CUDA_OK;
+}
+inline int cuda_fail(const char *what, cudaError_t e) {
+    set_last_error(std::string(what) + ": " + cudaGetErrorString(e));
+    return TC_CUDA_FAIL;
+}
+
+// The context's device current for a call, the caller's afterwards.
+struct CurrentDevice {
+    int previous = -1;
+    explicit CurrentDevice(int device) {
+        if (cudaGetDevice(&previous) != cudaSuccess) previous = -1;
+        if (previous != device) cudaSetDevice(device);
+        else previous = -1;
+    }
+    ~CurrentDevice() {
+        if (previous >= 0) cudaSetDevice(previous);
+    }
+};
+
+// Checks of the arguments; nullptr: fine.
 const char *check_cache(const tc_paged_cache *c, CacheView &v);
 const char *check_batch(const tc_paged_batch *b, BatchView &v);
 // Whether [a][b] rows of `width` elements at strides ld_a, ld_b share elements.

@@ -344,15 +344,6 @@ cudaError_t launch_heads(HeadsParams &p, bool half, bool wide, int sm_count, cud
     return launch_sized<T, 4, APPEND>(p, half, wide, sm_count, s);
 }
 
-int fail(const char *reason) {
-    set_last_error(reason);
-    return TC_CUDA_FAIL;
-}
-int ok() {
-    set_last_error("");
-    return TC_CUDA_OK;
-}
-
 HeadsView view_of(const tc_heads *h) {
     return {h->x, h->out, h->weight, h->ld_token, h->ld_head, h->ld_out_token, h->ld_out_head, h->n_heads};
 }
@@ -426,23 +417,6 @@ const char *take_norm(HeadsParams &p, int rms_norm, float eps, uint32_t head_dim
     p.head_dim = head_dim;
     return nullptr;
 }
-
-int cuda_fail(const char *what, cudaError_t e) {
-    set_last_error(std::string(what) + ": " + cudaGetErrorString(e));
-    return TC_CUDA_FAIL;
-}
-
-struct CurrentDevice {
-    int previous = -1;
-    explicit CurrentDevice(int device) {
-        if (cudaGetDevice(&previous) != cudaSuccess) previous = -1;
-        if (previous != device) cudaSetDevice(device);
-        else previous = -1;
-    }
-    ~CurrentDevice() {
-        if (previous >= 0) cudaSetDevice(previous);
-    }
-};
 
 }  // namespace
 

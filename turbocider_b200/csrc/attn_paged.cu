@@ -554,19 +554,6 @@ bool encode_cache(CUtensorMap *map, const uint16_t *base, const CacheView &c, ui
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int fail(const char *reason) {
-    set_last_error(reason);
-    return TC_CUDA_FAIL;
-}
-int ok() {
-    set_last_error("");
-    return TC_CUDA_OK;
-}
-int cuda_fail(const char *what, cudaError_t e) {
-    set_last_error(std::string(what) + ": " + cudaGetErrorString(e));
-    return TC_CUDA_FAIL;
-}
-
 // Grows the context's split workspace; the counters start at zero and every
 // complete kernel leaves them so.
 int ensure_split(tc_cuda_ctx *ctx, size_t floats, size_t counters, cudaStream_t s) {
@@ -594,18 +581,6 @@ int ensure_split(tc_cuda_ctx *ctx, size_t floats, size_t counters, cudaStream_t 
     }
     return TC_CUDA_OK;
 }
-
-struct CurrentDevice {
-    int previous = -1;
-    explicit CurrentDevice(int device) {
-        if (cudaGetDevice(&previous) != cudaSuccess) previous = -1;
-        if (previous != device) cudaSetDevice(device);
-        else previous = -1;
-    }
-    ~CurrentDevice() {
-        if (previous >= 0) cudaSetDevice(previous);
-    }
-};
 
 int attend(tc_cuda_ctx *ctx, const tc_paged_cache *cache, const tc_paged_batch *batch, const tc_attention *a,
            cudaStream_t s) {
