@@ -207,6 +207,10 @@ def test_refusals(ctx):
     refused("overlapping cache", tcc.paged_attention, ctx, tcc.PagedCache(shared, shared), batch, q)
     refused("f16 or bf16", tcc.paged_attention, ctx, tcc.PagedCache(k.float(), v.float()), batch, q.float())
     refused("same shape", tcc.PagedCache, k, v[:, :, :8])
+    refused("device tensors", tcc.PagedCache, k.cpu(), v.cpu())
+    refused("device", tcc.PagedBatch, offsets.cpu(), lengths, table, 2, 30)
+    refused("device", tcc.PagedBatch, offsets, lengths, table.cpu(), 2, 30)
+    refused("context's device", tcc.paged_attention, ctx, cache, batch, q.cpu())
     refused("int32", tcc.PagedBatch, offsets.long(), lengths, table, 2, 30)
     refused("rows", tcc.PagedBatch, offsets[:1], lengths, table, 2, 30)
     assert ctx.status() == 0

@@ -579,11 +579,17 @@ def _stream_of(ctx: Context, stream) -> int:
     return getattr(stream, "cuda_stream", stream)
 
 
-def _ints(t, what: str, dims: int) -> int:
-    """Address of a contiguous int32 device tensor."""
-    if t.dtype is not _torch_once().i32 or not t.is_cuda or t.dim() != dims or not t.is_contiguous():
-        raise BackendError(f"{what} must be a contiguous int32 device tensor of {dims} dimension(s)")
+def _ints(t, what: str, dims: int, device: int) -> int:
+    """Address of a contiguous int32 tensor on `device`."""
+    if t.dtype is not _torch_once().i32 or t.get_device() != device or t.dim() != dims or not t.is_contiguous():
+        raise BackendError(f"{what} must be a contiguous int32 tensor of {dims} dimension(s) on the others' device")
     return t.data_ptr()
+
+
+def _same_device(device: int, *parts) -> None:
+    for part in parts:
+        if part is not None and part.device != device:
+            raise BackendError("every tensor of a call must be on the context's device")
 
 
 def rope_freqs(rotary_dim: int, theta: float = 10000.0, scaling: str = "plain", factor: float = 1.0,
@@ -609,28 +615,29 @@ class Rope:
     token's place in its cache.  layout: "half" (pairs i, i + rotary_dim / 2)
     or "interleaved" (2i, 2i + 1).  sections: pairs of each axis."""
 
-    __slots__ = ("c", "freq", "positions")
+    __slots__ = ("c", "freq", "positions", "device")
 
     def __init__(self, freq, positions=None, layout: str = "half", sections=None, amplitude: float = 1.0):
-        if freq.dtype is not _torch_once().f64 or not freq.is_cuda or freq.dim() != 1 or not freq.is_contiguous():
+        device = self.device = freq.get_device()
+        if freq.dtype is not _torch_once().f64 or device < 0 or freq.dim() != 1 or not freq.is_contiguous():
             raise BackendError("freq must be a contiguous float64 device vector")
-        if layout not in _ROPE_LAYOUTS:
+        layout = _ROPE_LAYOUTS.get(layout)
+        if layout is None:
             raise BackendError("invalid rotation layout")
-        axes, dims, pairs = 1, 1, freq.numel()
-        if positions is not None and positions.dim() == 2:
-            axes, dims = positions.shape[1], 2
+        c, pairs, axes = _Rope(), freq.numel(), 1
+        self.freq, self.positions, self.c = freq, positions, c
+        if positions is not None:
+            shape = positions.shape
+            if len(shape) == 2:
+                axes = shape[1]
+            c.positions = _ints(positions, "positions", 2 if len(shape) == 2 else 1, device)
         if axes != (1 if sections is None else len(sections)) or not 1 <= axes <= 4:
             raise BackendError("one section for each of 1 to 4 position axes")
-        self.freq, self.positions = freq, positions
-        c = self.c = _Rope()
-        c.freq = freq.data_ptr()
-        if positions is not None:
-            c.positions = _ints(positions, "positions", dims)
-        c.rotary_dim, c.layout, c.n_axes, c.amplitude = 2 * pairs, _ROPE_LAYOUTS[layout], axes, amplitude
         if axes > 1:
             c.sections = tuple(sections) + (0,) * (4 - axes)
         elif sections is not None and sections[0] != pairs:
             raise BackendError("the sections must add up to rotary_dim / 2")
+        c.freq, c.rotary_dim, c.layout, c.n_axes, c.amplitude = freq.data_ptr(), 2 * pairs, layout, axes, amplitude
 
 
 class PagedCache:
@@ -639,12 +646,13 @@ class PagedCache:
     token_major=True [pages, page_size, heads, head_dim], of the same strides,
     the last one contiguous."""
 
-    __slots__ = ("c", "k", "v", "dtype", "head_dim", "n_heads", "page_size")
+    __slots__ = ("c", "k", "v", "dtype", "head_dim", "n_heads", "page_size", "device")
 
     def __init__(self, k, v, token_major: bool = False):
         if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype:
             raise BackendError("keys and values must be 4-dimensional tensors of the same shape, strides and type")
-        if not k.is_cuda or k.device != v.device or k.stride(3) != 1:
+        self.device = k.get_device()
+        if self.device < 0 or v.get_device() != self.device or k.stride(3) != 1:
             raise BackendError("the cache must be device tensors with a contiguous head dimension")
         token, head = (1, 2) if token_major else (2, 1)
         self.k, self.v, self.dtype = k, v, k.dtype
@@ -661,36 +669,39 @@ class PagedBatch:
     ones included) and page_table [requests, width]; max_new and max_length
     bound the new tokens and the length of every request."""
 
-    __slots__ = ("c", "tensors")
+    __slots__ = ("c", "tensors", "device")
 
     def __init__(self, new_offsets, lengths, page_table, max_new: int, max_length: int):
         n, shape, strides = lengths.numel(), page_table.shape, page_table.stride()
         if len(shape) != 2 or shape[0] != n or new_offsets.numel() != n + 1:
             raise BackendError("new_offsets, lengths and page_table must have requests + 1, requests and requests rows")
-        if page_table.dtype is not _torch_once().i32 or not page_table.is_cuda or (strides[1] != 1 and shape[1] > 1):
+        device = self.device = page_table.get_device()
+        if page_table.dtype is not _torch_once().i32 or device < 0 or (strides[1] != 1 and shape[1] > 1):
             raise BackendError("page_table must be an int32 device tensor with contiguous rows")
         if max_new < 0 or max_length < 0:
             raise BackendError("max_new and max_length must not be negative")
         self.tensors = (new_offsets, lengths, page_table)
         c = self.c = _PagedBatch()
-        c.new_offsets, c.lengths = _ints(new_offsets, "new_offsets", 1), _ints(lengths, "lengths", 1)
+        c.new_offsets, c.lengths = _ints(new_offsets, "new_offsets", 1, device), _ints(lengths, "lengths", 1, device)
         c.page_table, c.n_seq, c.table_width = page_table.data_ptr(), n, shape[1]
         c.ld_table = strides[0] if n > 1 else shape[1]
         c.max_new, c.max_length = max_new, max_length
 
 
-def _heads(x, out, weight, what: str, fresh: bool = False):
-    """(struct tc_heads, out) of a [tokens, heads, head_dim] device tensor;
-    fresh: a contiguous result is allocated where out is None."""
+def _heads(device: int, x, out, weight, what: str, fresh: bool = False):
+    """(struct tc_heads, out) of a [tokens, heads, head_dim] tensor on the
+    context's device; fresh: a contiguous result is allocated where out is
+    None."""
     shape, strides = x.shape, x.stride()
-    if len(shape) != 3 or not x.is_cuda or (strides[2] != 1 and shape[2] > 1):
-        raise BackendError(f"{what} must be a device tensor [tokens, heads, head_dim] with a contiguous last dimension")
-    tokens, heads, dim = shape
+    if len(shape) != 3 or x.get_device() != device or (strides[2] != 1 and shape[2] > 1):
+        raise BackendError(f"{what} must be [tokens, heads, head_dim] with a contiguous last dimension on the "
+                           "context's device")
+    _, heads, dim = shape
     h = _Heads()
     h.x, h.n_heads, h.ld_token, h.ld_head = x.data_ptr(), heads, strides[0], strides[1]
     if out is not None:
         strides = out.stride()
-        if out.shape != shape or out.dtype is not x.dtype or out.get_device() != x.get_device() or \
+        if out.shape != shape or out.dtype is not x.dtype or out.get_device() != device or \
                 (strides[2] != 1 and dim > 1):
             raise BackendError(f"the result of {what} must have its shape, type and device")
         h.out, h.ld_out_token, h.ld_out_head = out.data_ptr(), strides[0], strides[1]
@@ -698,8 +709,8 @@ def _heads(x, out, weight, what: str, fresh: bool = False):
         out = _torch.empty_like(x, memory_format=_torch.dense)
         h.out, h.ld_out_token, h.ld_out_head = out.data_ptr(), heads * dim, dim
     if weight is not None:
-        if weight.dtype is not _torch.f32 or weight.dim() != 1 or weight.numel() != dim or \
-                not weight.is_contiguous() or weight.get_device() != x.get_device():
+        if weight.dtype is not _torch.f32 or weight.shape != (dim,) or not weight.is_contiguous() or \
+                weight.get_device() != device:
             raise BackendError("norm weights must be float32 device vectors of head_dim elements")
         h.weight = weight.data_ptr()
     return h, out
@@ -712,12 +723,15 @@ def qk_norm_rope(ctx: Context, q, k=None, rope: Rope | None = None, q_weight=Non
     launch.  Weights: f32 [head_dim].  q_out / k_out may be q / k.  Returns
     (q_out, k_out)."""
     dtype, hk = _dtype_id(q), None
-    hq, q_out = _heads(q, q_out, q_weight, "q", True)
+    device = ctx.device
+    hq, q_out = _heads(device, q, q_out, q_weight, "q", True)
     tokens, _, dim = q.shape
     if k is not None:
-        if k.dtype is not q.dtype or k.get_device() != q.get_device() or k.shape[0] != tokens or k.shape[2] != dim:
-            raise BackendError("q and k must share their type, device, tokens and head_dim")
-        hk, k_out = _heads(k, k_out, k_weight, "k", True)
+        shape = k.shape
+        if k.dtype is not q.dtype or shape[0] != tokens or shape[2] != dim:
+            raise BackendError("q and k must share their type, tokens and head_dim")
+        hk, k_out = _heads(device, k, k_out, k_weight, "k", True)
+    _same_device(device, rope)
     if rope is not None and rope.positions is not None and rope.positions.shape[0] != tokens:
         raise BackendError("one position for each token")
     _check(lib().tc_cuda_qk_norm_rope(ctx.handle, hq, hk, tokens, dim, dtype, eps is not None, eps or 0.0,
@@ -730,7 +744,7 @@ def kv_append(ctx: Context, cache: PagedCache, batch: PagedBatch, k, v, rope: Ro
     """Writes the step's keys (normed with eps not None, rotated with rope)
     and values [tokens, heads, head_dim] to the cache and, in the same launch,
     norms and rotates the queries.  Returns q_out (None without q)."""
-    shape = k.shape
+    shape, device = k.shape, ctx.device
     if k.dtype is not cache.dtype or v.dtype is not cache.dtype or v.shape != shape or shape[2] != cache.head_dim:
         raise BackendError("keys and values must have the cache's type and head_dim")
     tokens, hq = shape[0], None
@@ -739,10 +753,11 @@ def kv_append(ctx: Context, cache: PagedCache, batch: PagedBatch, k, v, rope: Ro
     if q is not None:
         if q.dtype is not cache.dtype or q.shape[0] != tokens or q.shape[2] != shape[2]:
             raise BackendError("queries must have the cache's type and head_dim and one row for each key")
-        hq, q_out = _heads(q, q_out, q_weight, "q", True)
+        hq, q_out = _heads(device, q, q_out, q_weight, "q", True)
+    _same_device(device, cache, batch, rope)
     batch.c.n_tokens = tokens
-    _check(lib().tc_cuda_kv_append(ctx.handle, cache.c, batch.c, _heads(k, None, k_weight, "k")[0],
-                                   _heads(v, None, None, "v")[0], hq, eps is not None, eps or 0.0,
+    _check(lib().tc_cuda_kv_append(ctx.handle, cache.c, batch.c, _heads(device, k, None, k_weight, "k")[0],
+                                   _heads(device, v, None, None, "v")[0], hq, eps is not None, eps or 0.0,
                                    None if rope is None else rope.c, _stream_of(ctx, stream)))
     return q_out if q is not None else None
 
@@ -755,21 +770,26 @@ def paged_attention(ctx: Context, cache: PagedCache, batch: PagedBatch, q, scale
     Returns out, or (out, lse) with lse f32 [tokens, heads]."""
     t = _torch_once()
     shape, strides = q.shape, q.stride()
-    if len(shape) != 3 or q.dtype is not cache.dtype or q.get_device() != cache.k.get_device() or \
-            shape[2] != cache.head_dim or strides[2] != 1:
-        raise BackendError("queries must be [tokens, heads, head_dim] of the cache's type, device and head_dim")
+    device = ctx.device
+    if len(shape) != 3 or q.dtype is not cache.dtype or q.get_device() != device or shape[2] != cache.head_dim or \
+            strides[2] != 1:
+        raise BackendError("queries must be [tokens, heads, head_dim] of the cache's type and head_dim on the "
+                           "context's device")
     a = _Attention()
     a.q, a.ld_q_token, a.ld_q_head, a.n_heads = q.data_ptr(), strides[0], strides[1], shape[1]
     if out is None:
         out = t.empty_like(q, memory_format=t.dense)
-    strides = out.stride()
-    if out.shape != shape or out.dtype is not q.dtype or out.get_device() != q.get_device() or strides[2] != 1:
-        raise BackendError("the result must have the queries' shape, type and device")
+        strides = (shape[1] * shape[2], shape[2])
+    else:
+        strides = out.stride()
+        if out.shape != shape or out.dtype is not q.dtype or out.get_device() != device or strides[2] != 1:
+            raise BackendError("the result must have the queries' shape, type and device")
     a.out, a.ld_out_token, a.ld_out_head = out.data_ptr(), strides[0], strides[1]
     if return_lse:
         lse = t.empty(shape[:2], dtype=t.f32, device=q.device)
         a.lse = lse.data_ptr()
     a.causal, a.window, a.scale = causal, window, shape[2] ** -0.5 if scale is None else scale
+    _same_device(device, cache, batch)
     batch.c.n_tokens = shape[0]
     _check(lib().tc_cuda_paged_attention(ctx.handle, cache.c, batch.c, a, _stream_of(ctx, stream)))
     return (out, lse) if return_lse else out
