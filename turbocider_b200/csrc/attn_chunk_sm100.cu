@@ -27,7 +27,7 @@
 // TMEM: S_0, S_1 (two halves of 64 columns each), O_0, O_1 (head_dim each).
 // Blocks of rows go heaviest first (last rows first).  With few blocks the keys
 // are split over CTAs: partial results (column-major, so that the 128 threads of
-// a tile store and load whole lines) and the last to finish joins them in order.
+// a tile store whole lines), which a second kernel joins in order.
 //
 // What bounds it: the GPU's 1000 W.  2 x 4224 image tokens, 30 heads of 128, f16:
 // 557 us (985 TFLOP/s) in the first milliseconds, 614 us (892 TFLOP/s; 66 % of
@@ -176,13 +176,10 @@ constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
 __device__ __forceinline__ uint32_t desc_low(uint32_t saddr, uint32_t next) { return (saddr >> 4) | (next << 16); }
 __device__ __forceinline__ uint64_t desc(uint32_t low) { return (uint64_t)kDescHigh << 32 | low; }
 
-// Barrier of the 256 softmax threads.
-__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
-
 // What a CTA works on; the same in every thread.
 struct Work {
     Request rq;
-    uint32_t b, h, part, group_index, n_split, split;
+    uint32_t b, h, part, n_split, split;
     int32_t row0, n_rows;
     int32_t lo[2], hi[2];     // keys that tile i's rows see, within the CTA's share
     int32_t first[2], last[2];   // its half-steps of 64 keys (tile i has none: first == last)
@@ -195,12 +192,10 @@ __device__ __forceinline__ bool cut_step(const Work &w, int32_t j) {
     return j * kChunkKeys < w.seen_lo || (j + 1) * kChunkKeys > w.seen_hi;
 }
 
-__device__ __forceinline__ bool find_work(const AttnParams &p, Work &w) {
-    uint32_t id = blockIdx.x;
-    w.h = id % p.n_kv;
-    id /= p.n_kv;
-    w.split = id % p.splits;
-    const uint32_t blk = p.n_blocks - 1 - id / p.splits;
+// Share `split` of block `blk` of rows and cache head h; false: there is none.
+__device__ __forceinline__ bool find_work(const AttnParams &p, uint32_t blk, uint32_t h, uint32_t split, Work &w) {
+    w.h = h;
+    w.split = split;
     // Request b's blocks begin at first(b) = rows before it / 256 + b: that
     // leaves room for its partly filled one.
     auto first_block = [&](uint32_t b) {
@@ -266,8 +261,7 @@ __device__ __forceinline__ bool find_work(const AttnParams &p, Work &w) {
     }
     w.seen_lo = min(w.first[0] < w.last[0] ? w.lo[0] : 0x7fffffff, w.first[1] < w.last[1] ? w.lo[1] : 0x7fffffff);
     w.seen_hi = max(w.hi[0], w.hi[1]);
-    w.group_index = blk * p.n_kv + w.h;
-    w.part = w.group_index * p.splits + w.split;
+    w.part = (blk * p.n_kv + w.h) * p.splits + w.split;
     return true;
 }
 
@@ -313,7 +307,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     // (as the last it waited about 500 cycles for its turn at every barrier).
     const uint32_t warp = (threadIdx.x / 32 + 8) % 12, lane = threadIdx.x % 32, tid = warp * 32 + lane;
     Work w;
-    if (!find_work(p, w)) return;
+    {
+        const uint32_t id = blockIdx.x / p.n_kv;   // heaviest blocks (last rows) first
+        if (!find_work(p, p.n_blocks - 1 - id / p.splits, blockIdx.x % p.n_kv, id % p.splits, w)) return;
+    }
     const uint32_t bars = su32(smem + L::bar_off);
     auto kv_full = [&](uint32_t i) { return bars + 8 * i; };
     auto kv_empty = [&](uint32_t i) { return bars + 8 * (L::stages + i); };
@@ -322,7 +319,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto pv_done = [&](uint32_t i, uint32_t h) { return bars + 8 * (2 * L::stages + 8 + 2 * i + h); };
     const uint32_t q_full = bars + 8 * (2 * L::stages + 12), fin = q_full + 8, v_fixed = fin + 8;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + L::misc_off);
-    uint32_t *last_flag = tmem_slot + 1;
 
     if (tid == 0) {
         for (uint32_t i = 0; i < L::stages; ++i) {
@@ -628,47 +624,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
         }
-        if (w.n_split > 1) {
-            // ---- the share that finishes last adds them all, in order
-            __threadfence();
-            softmax_sync();
-            if (tid == 0) {
-                const uint32_t before = atomicAdd(p.counters + w.group_index, 1u);
-                *last_flag = before + 1 == w.n_split;
-                if (before + 1 == w.n_split) p.counters[w.group_index] = 0u;
-            }
-            softmax_sync();
-            if (*last_flag && valid) {
-            __threadfence();
-            const uint64_t part0 = (uint64_t)w.group_index * p.splits;
-            const float2 *ml = reinterpret_cast<const float2 *>(p.ws) + part0 * kChunkRows + tid;
-            const float *po = p.ws + p.ws_ml + part0 * DP * kChunkRows + tid;
-            float mm = -INFINITY, ll = 0.f;
-            for (uint32_t s = 0; s < w.n_split; ++s) mm = fmaxf(mm, __ldcg(ml + (uint64_t)s * kChunkRows).x);
-            const float base = mm == -INFINITY ? 0.f : mm;
-            for (uint32_t s = 0; s < w.n_split; ++s) {
-                const float2 v = __ldcg(ml + (uint64_t)s * kChunkRows);
-                ll += ex2(v.x - base) * v.y;
-            }
-            if (p.lse)
-                p.lse[token * (p.n_kv * p.group) + head] =
-                    ll == 0.f ? -INFINITY : (mm + log2f(ll)) * 0.693147180559945309f;
-            const float inv = ll == 0.f ? 0.f : 1.f / ll;
-        #pragma unroll 1
-            for (uint32_t k = 0; k < DP; k += 32) {
-                float acc[32] = {};
-                for (uint32_t s = 0; s < w.n_split; ++s) {
-                    const float2 v = __ldcg(ml + (uint64_t)s * kChunkRows);
-                    const float a = ex2(v.x - base);
-                    if (v.y == 0.f) continue;   // it saw nothing (a NaN sum is kept)
-        #pragma unroll
-                    for (uint32_t e = 0; e < 32; ++e)
-                        acc[e] = fmaf(a, __ldcg(po + ((uint64_t)s * DP + k + e) * kChunkRows), acc[e]);
-                }
-                store_row32<BF16>(p, out, k, acc, inv);
-            }
-            }
-        }
     }
 
     tc_fence_before();
@@ -676,6 +631,64 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 8) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::tmem_cols));
+    }
+}
+
+constexpr uint32_t kJoinRows = 32;
+
+// Adds the shares of 32 rows in order.  A warp takes DP / 8 columns, a lane a
+// row, so that every load is a whole line of the column-major partial results.
+// (Joined by the CTA that finished last, 16 shares of one block took 45 us.)
+template <int DP, bool BF16>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ AttnParams p) {
+    constexpr uint32_t cols = DP / 8;
+    __shared__ float2 stat[kChunkShares][kJoinRows];   // maximum and sum of a share's rows
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, r = blockIdx.y * kJoinRows + lane;
+    Work w;
+    if (!find_work(p, blockIdx.x / p.n_kv, blockIdx.x % p.n_kv, 0, w) || w.n_split == 1) return;
+    const float2 *ml = reinterpret_cast<const float2 *>(p.ws) + (uint64_t)w.part * kChunkRows + r;
+    for (uint32_t s = warp; s < w.n_split; s += 8) stat[s][lane] = ml[(uint64_t)s * kChunkRows];
+    __syncthreads();
+    const int32_t row = w.row0 + (int32_t)r;
+    if (row >= w.n_rows) return;
+    float m = -INFINITY, l = 0.f;
+    for (uint32_t s = 0; s < w.n_split; ++s) m = fmaxf(m, stat[s][lane].x);
+    const float base = m == -INFINITY ? 0.f : m;
+    const float *po = p.ws + p.ws_ml + ((uint64_t)w.part * DP + warp * cols) * kChunkRows + r;
+    float acc[cols] = {};
+#pragma unroll 2
+    for (uint32_t s = 0; s < w.n_split; ++s) {
+        const float2 v = stat[s][lane];
+        const float a = v.y == 0.f ? 0.f : ex2(v.x - base);   // (a share that saw nothing has written nothing)
+        l += a * v.y;
+#pragma unroll
+        for (uint32_t e = 0; e < cols; ++e) {
+            const float x = po[((uint64_t)s * DP + e) * kChunkRows];
+            acc[e] = v.y == 0.f ? acc[e] : fmaf(a, x, acc[e]);
+        }
+    }
+    const uint64_t token = (uint64_t)w.rq.first + row / (int32_t)p.group;
+    const uint32_t head = w.h * p.group + row % (int32_t)p.group;
+    if (p.lse && warp == 0)
+        p.lse[token * (p.n_kv * p.group) + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147180559945309f;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    uint16_t *o = p.out + token * p.ld_out_token + head * p.ld_out_head;
+#pragma unroll
+    for (uint32_t e = 0; e < cols; e += 8) {
+        const uint32_t d = warp * cols + e;
+        if (d >= p.head_dim) break;
+        uint32_t u[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) u[k] = pack16<BF16>(acc[e + 2 * k] * inv, acc[e + 2 * k + 1] * inv);
+        if (p.out_wide) {
+            *reinterpret_cast<uint4 *>(o + d) = make_uint4(u[0], u[1], u[2], u[3]);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                o[d + 2 * k] = (uint16_t)u[k];
+                o[d + 2 * k + 1] = (uint16_t)(u[k] >> 16);
+            }
+        }
     }
 }
 
@@ -690,6 +703,8 @@ cudaError_t launch_inst(const CUtensorMap &km, const CUtensorMap &vm, const Attn
     });
     if (e != cudaSuccess) return e;
     kernel<<<p.n_blocks * p.n_kv * p.splits, kThreads, L::bytes, s>>>(km, vm, p);
+    if (p.splits > 1)
+        join_kernel<DP, BF16><<<dim3(p.n_blocks * p.n_kv, kChunkRows / kJoinRows), 256, 0, s>>>(p);
     return cudaGetLastError();
 }
 

@@ -33,6 +33,7 @@ struct AttnParams {
 // Chunks of many rows (attn_chunk_sm100.cu), head_dim at most 128.
 constexpr int kChunkRows = 256;      // rows of a CTA: two tensor-core tiles
 constexpr int kChunkKeys = 128;      // keys of a step
+constexpr uint32_t kChunkShares = 64;   // shares of the keys, at most
 cudaError_t launch_chunk(const CUtensorMap &km, const CUtensorMap &vm, const AttnParams &p, bool bf16,
                          cudaStream_t s);
 

@@ -647,15 +647,16 @@ int attend(tc_cuda_ctx *ctx, const tc_paged_cache *cache, const tc_paged_batch *
         if (p.scale_log2 < 1e-30f) p.scale_log2 = 1e-30f;   // 0 * -inf would lose the mask
         // Shares of the keys: as many CTAs as make the busiest SM's work least,
         // in steps of 128 keys plus kCtaSteps for what a CTA does besides, one
-        // CTA per SM, no share under kLeastSteps.
-        constexpr uint64_t kCtaSteps = 3, kLeastSteps = 3;
+        // CTA per SM, and the time to join the shares (2 us and 0.5 us a share,
+        // in steps of 2 us); no share under kLeastSteps.
+        constexpr uint64_t kCtaSteps = 3, kLeastSteps = 2;
         const uint64_t steps = (span + kChunkKeys - 1) / kChunkKeys + 1;
         const uint64_t blocks = std::max<uint64_t>((rows + kChunkRows - 1) / kChunkRows, p.batch.n_seq);
         uint64_t best = ~0ull, share = steps;
-        for (uint64_t n = 1; n <= 64 && (n == 1 || steps / n >= kLeastSteps); ++n) {
+        for (uint64_t n = 1; n <= kChunkShares && (n == 1 || steps / n >= kLeastSteps); ++n) {
             const uint64_t each = (steps + n - 1) / n, real = (steps + each - 1) / each;
             const uint64_t waves = (blocks * c.n_heads * real + ctx->sm_count - 1) / ctx->sm_count;
-            const uint64_t cost = waves * (each + kCtaSteps + (real > 1 ? 1 : 0));
+            const uint64_t cost = 4 * waves * (each + kCtaSteps) + (real > 1 ? 4 + real : 0);
             if (cost < best) {
                 best = cost;
                 share = each;
@@ -667,9 +668,8 @@ int attend(tc_cuda_ctx *ctx, const tc_paged_cache *cache, const tc_paged_batch *
         if (p.splits > 1) {
             const uint64_t parts = (uint64_t)p.n_blocks * c.n_heads * p.splits * kChunkRows;
             p.ws_ml = parts * 2;
-            if (ensure_split(ctx, p.ws_ml + parts * dp, (size_t)p.n_blocks * c.n_heads, s)) return TC_CUDA_FAIL;
+            if (ensure_split(ctx, p.ws_ml + parts * dp, 0, s)) return TC_CUDA_FAIL;
             p.ws = ctx->attn_ws;
-            p.counters = ctx->attn_counters;
         }
         CUtensorMap km, vm;
         const uint32_t box = c.page_size < kChunkKeys ? c.page_size : kChunkKeys;
