@@ -29,16 +29,22 @@
 // are split over CTAs: partial results (column-major, so that the 128 threads of
 // a tile store whole lines), which a second kernel joins in order.
 //
-// What bounds it: the GPU's 1000 W.  2 x 4224 image tokens, 30 heads of 128, f16:
-// 557 us (985 TFLOP/s) in the first milliseconds, 614 us (892 TFLOP/s; 66 % of
-// what cuBLAS sustains) in a loop, where the cap lowers the clock from 1965 to
-// about 1700 MHz.  At full clock a step takes about 4500 cycles against 2048 of
-// the tensor cores and 2048 of the special-function units (exponentials): two
-// softmax warps per scheduler reach 10 of them in 100 cycles, not 12.5.
-// Tried and dropped: 128-key softmax steps with one issuer (3 % slower on
-// prompts, 3 % faster on long chunks), two threads per row, tiles taking turns
-// with the special-function units, a quarter of the exponentials by polynomial
-// (each 2 to 10 % slower on long chunks: more instructions, more power).
+// What bounds it (2 x 4224 image tokens, 30 heads of 128, f16; 493 us, 1111
+// TFLOP/s, in the first milliseconds).  A step takes about 3340 cycles, and as
+// many with the exponentials left out: the tensor cores work through four
+// products of 128 x 64 keys, which take as long as 128 x 128 ones would (every
+// product of a tile reads all its queries from shared memory), and two of
+// 128 x head_dim.  The special-function units are busy for 2048 of them (32768
+// exponentials).  Besides, a CTA costs about 8 us for finding its work, the
+// queries, the first product and the results.  In a loop the GPU's 1000 W cap
+// lowers the clock from 1965 to about 1700 MHz: 558 us (982 TFLOP/s, 72 % of
+// what cuBLAS sustains there).
+// Tried and dropped: one issuer and 128-key steps, where a tile waits for its
+// products (the same time on these, 2 % slower on prompts, 2 % faster on one long
+// chunk, 216 registers instead of 122); two threads per row; tiles taking turns
+// with the special-function units; a quarter or an eighth of the exponentials by
+// polynomial (faster by 1 % at best, 7 % slower on the long chunk, where the
+// power cap binds most).
 //
 // Every wait is bounded; on timeout the kernel sets TC_STATUS_TIMEOUT, drains
 // its copies and MMAs, frees TMEM and returns.  No multicast.
@@ -302,9 +308,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     using L = ChunkLayout<DP>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    // Warps of the block in the order of their roles: the issuing warp is the
-    // block's first, since the scheduler favours the oldest of the ready warps
-    // (as the last it waited about 500 cycles for its turn at every barrier).
+    // Warps by role, as listed above (the block's first four are 8 to 11).
     const uint32_t warp = (threadIdx.x / 32 + 8) % 12, lane = threadIdx.x % 32, tid = warp * 32 + lane;
     Work w;
     {

@@ -10,10 +10,15 @@
 // power-of-two group of lanes that gives each lane one unit of 16 elements (8
 // for f32 and for odd sizes): two chunks half a rotary width apart for the
 // half layout, half a head apart for the interleaved one (whole sectors per
-// access), so that both members of every pair are in one lane, the rotation needs no exchange and the norm one
-// butterfly over the group.  A warp takes one token and some or all of its
-// heads, kBatch for each lane group at a time; the token's sines and cosines are
-// formed once per warp.
+// access), so that both members of every pair are in one lane, the rotation
+// needs no exchange and the norm one butterfly over the group.  A warp takes one
+// token and some or all of its heads, kBatch for each lane group at a time; the
+// token's sines and cosines are formed once per warp, the norm's weights folded
+// into them, and the arithmetic is packed two fp32 to an operation: with 8-byte
+// chunks and plain arithmetic half of the time went into issuing instructions.
+// 8448 tokens x 60 heads of 128 (260 MB): 53 us, 4.9 TB/s; appending 281 MB:
+// 57.5 us.  More warps or heads in flight, batches read ahead, or a token split
+// over warps were each slower (52 to 79 us).
 //
 // The angle: freq / 2 pi is held as a 64-bit binary fraction of a turn and
 // multiplied by the position modulo 2^64, i.e. modulo one turn and exactly,

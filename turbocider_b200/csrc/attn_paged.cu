@@ -6,15 +6,21 @@
 // read once for all of them.  This file has the kernel for few rows (single
 // tokens, a few drafted ones): bytes bound, the floor is one read of K and V.
 //
-// A CTA takes up to 16 rows (one mma.sync tile; with so few rows the tensor
-// work is a small part of the memory time, so the padding costs nothing) of
-// one cache head and one chunk of the cache; its four warps take 16-key steps
-// in turn, each with its own running maximum, sum and output in registers, so
-// the loop has no CTA-wide synchronisation.  Each warp keeps a ring of TMA
-// boxes in flight (64 elements x up to 16 tokens of a page, 128-byte swizzle,
-// conflict-free for ldmatrix).  The warps' results are joined in shared
-// memory, the chunks' by the CTA that finishes last (partial outputs in the
-// workspace, added in chunk order, so the result does not depend on timing).
+// A CTA takes up to 16, 32 or 64 rows (mma.sync tiles of 16; with so few rows the
+// tensor work is a small part of the memory time, so the padding costs nothing)
+// of one cache head and one chunk of the cache; its four warps take steps of 16
+// or 32 keys in turn, each with its own running maximum, sum and output in
+// registers, so the loop has no CTA-wide synchronisation.  Each warp keeps a
+// ring of TMA boxes in flight (64 elements x up to a step's tokens of a page,
+// 128-byte swizzle, conflict-free for ldmatrix), a lane issuing each.  The warps'
+// results are joined in shared memory, the chunks' by the CTA that finishes last
+// (partial outputs in the workspace, added in chunk order, so the result does
+// not depend on timing).
+//
+// A decode step of 96 requests, 1.5 GB of cache: 236 us, 6.48 TB/s (98.8 % of the
+// measured copy).  One token over 3001 positions (12 MB): 9.6 us, bound by one
+// CTA's chain: 0.9 us to its pages, 2 us to the first keys, 2 us of steps, 0.6 us to
+// join the warps, 1 us for the arrival, 1.5 us to add the shares.
 //
 // Probabilities are rounded to the cache's 16-bit type for the P V product
 // (its relative error, 2^-9 or 2^-12 an element, averages out over the keys);
