@@ -552,7 +552,8 @@ int tc_cuda_kv_append(tc_cuda_ctx *ctx, const tc_paged_cache *cache, const tc_pa
  * the same request; past the request's length nothing is read into results.
  * Long caches are split over CTAs with partial results in the context's
  * workspace, which grows on demand (outside stream captures: make the first
- * call of the largest sizes before capturing). */
+ * call of the largest sizes before capturing); calls on several streams must
+ * be ordered by the caller, or use a context each. */
 typedef struct tc_attention {
     const void *q;
     void *out;

@@ -239,3 +239,9 @@ def test_offsets_past_32_bits(ctx):
         want, _, tol, _ = ac.attention_ref(q, [(new, n)], ks, vs, dim ** -0.5, True, 0)
         ac.close(y, want, tol)
     assert ctx.status() == 0
+
+
+@pytest.mark.parametrize("window", [2**31 - 1, 2**31 + 5, 2**32 + 3])
+@pytest.mark.parametrize("causal", [True, False])
+def test_windows_past_32_bits_hide_nothing(ctx, causal, window):
+    attend(ctx, [(1, 90), (40, 90)], 16, 4, 2, 64, BF, seed=31, causal=causal, window=window)

@@ -219,3 +219,25 @@ def test_refusals(ctx):
     refused("one row for each key", tcc.kv_append, ctx, cache, batch, x, x, q=x[:2])
     assert tcc.qk_norm_rope(ctx, x[:0])[0].shape == (0, 2, 64)
     assert ctx.status() == 0
+
+
+def test_refuses_other_ranks_and_wide_bounds(ctx):
+    """Tensors that are not three-dimensional and bounds past 32 bits are refused, not read or cut off."""
+    from turbocider_b200 import cuda as tcc
+    x = ac.normal(ac.gen(7), (4, 2, 64), BF)
+    kc = torch.zeros((4, 2, 16, 64), dtype=BF, device="cuda")
+    cache = tcc.PagedCache(kc, kc.clone())
+    offsets = torch.tensor([0, 4], dtype=torch.int32, device="cuda")
+    length, table = offsets[1:], torch.zeros((1, 1), dtype=torch.int32, device="cuda")
+    batch = tcc.PagedBatch(offsets, length, table, 4, 4)
+    flat = x.reshape(4, 128)
+    for call in (lambda: tcc.qk_norm_rope(ctx, flat), lambda: tcc.qk_norm_rope(ctx, x, flat),
+                 lambda: tcc.kv_append(ctx, cache, batch, flat, flat),
+                 lambda: tcc.kv_append(ctx, cache, batch, x, flat),
+                 lambda: tcc.kv_append(ctx, cache, batch, x, x, q=flat),
+                 lambda: tcc.paged_attention(ctx, cache, batch, flat),
+                 lambda: tcc.PagedBatch(offsets, length, table, 2**32 + 4, 4),
+                 lambda: tcc.PagedBatch(offsets, length, table, 4, 2**32 + 4)):
+        with pytest.raises(tcc.BackendError):
+            call()
+    assert not kc.any() and ctx.status() == 0

@@ -678,8 +678,8 @@ class PagedBatch:
         device = self.device = page_table.get_device()
         if page_table.dtype is not _torch_once().i32 or device < 0 or (strides[1] != 1 and shape[1] > 1):
             raise BackendError("page_table must be an int32 device tensor with contiguous rows")
-        if max_new < 0 or max_length < 0:
-            raise BackendError("max_new and max_length must not be negative")
+        if not (0 <= max_new < 2**32 and 0 <= max_length < 2**32):
+            raise BackendError("max_new and max_length must not be negative nor pass 32 bits")
         self.tensors = (new_offsets, lengths, page_table)
         c = self.c = _PagedBatch()
         c.new_offsets, c.lengths = _ints(new_offsets, "new_offsets", 1, device), _ints(lengths, "lengths", 1, device)
@@ -721,14 +721,15 @@ def qk_norm_rope(ctx: Context, q, k=None, rope: Rope | None = None, q_weight=Non
     """RMS norm over each head (eps None: no norm) and position rotation (rope
     None: none) of query and key heads [tokens, heads, head_dim] in one
     launch.  Weights: f32 [head_dim].  q_out / k_out may be q / k.  Returns
-    (q_out, k_out)."""
+    (q_out, k_out).  Results that are not passed in come from the current
+    stream's memory: with another `stream`, pass them or order the two."""
     dtype, hk = _dtype_id(q), None
     device = ctx.device
     hq, q_out = _heads(device, q, q_out, q_weight, "q", True)
     tokens, _, dim = q.shape
     if k is not None:
         shape = k.shape
-        if k.dtype is not q.dtype or shape[0] != tokens or shape[2] != dim:
+        if len(shape) != 3 or k.dtype is not q.dtype or shape[0] != tokens or shape[2] != dim:
             raise BackendError("q and k must share their type, tokens and head_dim")
         hk, k_out = _heads(device, k, k_out, k_weight, "k", True)
     _same_device(device, rope)
@@ -743,15 +744,18 @@ def kv_append(ctx: Context, cache: PagedCache, batch: PagedBatch, k, v, rope: Ro
               q_weight=None, k_weight=None, eps: float | None = None, q_out=None, stream=None):
     """Writes the step's keys (normed with eps not None, rotated with rope)
     and values [tokens, heads, head_dim] to the cache and, in the same launch,
-    norms and rotates the queries.  Returns q_out (None without q)."""
+    norms and rotates the queries.  Returns q_out (None without q; where it is
+    not passed in it comes from the current stream's memory, as with
+    qk_norm_rope)."""
     shape, device = k.shape, ctx.device
-    if k.dtype is not cache.dtype or v.dtype is not cache.dtype or v.shape != shape or shape[2] != cache.head_dim:
+    if k.dtype is not cache.dtype or v.dtype is not cache.dtype or v.shape != shape or len(shape) != 3 or \
+            shape[2] != cache.head_dim:
         raise BackendError("keys and values must have the cache's type and head_dim")
     tokens, hq = shape[0], None
     if rope is not None and rope.positions is not None and rope.positions.shape[0] != tokens:
         raise BackendError("one position for each token")
     if q is not None:
-        if q.dtype is not cache.dtype or q.shape[0] != tokens or q.shape[2] != shape[2]:
+        if q.dtype is not cache.dtype or len(q.shape) != 3 or q.shape[0] != tokens or q.shape[2] != shape[2]:
             raise BackendError("queries must have the cache's type and head_dim and one row for each key")
         hq, q_out = _heads(device, q, q_out, q_weight, "q", True)
     _same_device(device, cache, batch, rope)
@@ -767,7 +771,10 @@ def paged_attention(ctx: Context, cache: PagedCache, batch: PagedBatch, q, scale
     """softmax(scale q K^T) V of the step's queries [tokens, heads, head_dim]
     over each request's cache (scale None: head_dim ** -0.5); query heads share
     cache heads in equal groups.  window > 0: only positions nearer than that.
-    Returns out, or (out, lse) with lse f32 [tokens, heads]."""
+    Returns out, or (out, lse) with lse f32 [tokens, heads], of the current
+    stream's memory where they are not passed in, as with qk_norm_rope.  Calls
+    on one context share its workspace and follow one another in stream
+    order."""
     t = _torch_once()
     shape, strides = q.shape, q.stride()
     device = ctx.device
@@ -788,7 +795,8 @@ def paged_attention(ctx: Context, cache: PagedCache, batch: PagedBatch, q, scale
     if return_lse:
         lse = t.empty(shape[:2], dtype=t.f32, device=q.device)
         a.lse = lse.data_ptr()
-    a.causal, a.window, a.scale = causal, window, shape[2] ** -0.5 if scale is None else scale
+    # (positions stay below 2^30: a wider window hides as much as the widest one the struct holds)
+    a.causal, a.window, a.scale = causal, min(max(window, -1), 2**31 - 1), shape[2] ** -0.5 if scale is None else scale
     _same_device(device, cache, batch)
     batch.c.n_tokens = shape[0]
     _check(lib().tc_cuda_paged_attention(ctx.handle, cache.c, batch.c, a, _stream_of(ctx, stream)))
