@@ -447,7 +447,8 @@ int tc_gguf_validate_split(const tc_gguf *const *shards, uint32_t n);
  */
 
 /* Heads of one projection, as a [n_tokens][n_heads][head_dim] view.  `weight`
- * (f32 [head_dim], NULL = ones) is the norm's.  `out` may be `x` itself. */
+ * (f32 [head_dim], NULL = ones) is the norm's and not read without one.  `out`
+ * may be `x` itself. */
 typedef struct tc_heads {
     const void *x;
     void *out;

@@ -349,8 +349,9 @@ cudaError_t launch_heads(HeadsParams &p, bool half, bool wide, int sm_count, cud
     return launch_sized<T, 4, APPEND>(p, half, wide, sm_count, s);
 }
 
-HeadsView view_of(const tc_heads *h) {
-    return {h->x, h->out, h->weight, h->ld_token, h->ld_head, h->ld_out_token, h->ld_out_head, h->n_heads};
+// (the weight belongs to the norm: without one it has no part)
+HeadsView view_of(const tc_heads *h, int rms_norm) {
+    return {h->x, h->out, rms_norm ? h->weight : nullptr, h->ld_token, h->ld_head, h->ld_out_token, h->ld_out_head, h->n_heads};
 }
 
 // Units of a row can be moved by 16-byte accesses.
@@ -543,8 +544,8 @@ int tc_cuda_qk_norm_rope(tc_cuda_ctx *ctx, const tc_heads *q, const tc_heads *k,
                   chunked(h->out, h->ld_out_token, h->ld_out_head, item);
         }
         if ((uint64_t)q->n_heads + (k ? k->n_heads : 0) > 65535) return fail("too many heads");
-        p.q = view_of(q);
-        if (k) p.k = view_of(k);
+        p.q = view_of(q, rms_norm);
+        if (k) p.k = view_of(k, rms_norm);
         p.n_tokens = (uint32_t)n_tokens;
         p.status = ctx->status;
         CurrentDevice guard(ctx->device);
@@ -585,9 +586,9 @@ int tc_cuda_kv_append(tc_cuda_ctx *ctx, const tc_paged_cache *cache, const tc_pa
             if (h == q) vec = vec && chunked(h->out, h->ld_out_token, h->ld_out_head, 2);
         }
         if ((uint64_t)k->n_heads + v->n_heads + (q ? q->n_heads : 0) > 65535) return fail("too many heads");
-        p.k = view_of(k);
-        p.v = view_of(v);
-        if (q) p.q = view_of(q);
+        p.k = view_of(k, rms_norm);
+        p.v = view_of(v, 0);
+        if (q) p.q = view_of(q, rms_norm);
         p.n_tokens = p.batch.n_tokens;
         p.status = ctx->status;
         CurrentDevice guard(ctx->device);
