@@ -90,7 +90,30 @@ class AttentionBlock:
 
     def __call__(self, x, batch: tcc.PagedBatch, stream=None):
         """x: bf16 [tokens, hidden] of the step's new tokens; returns the
-        block's output [tokens, out.n] (bf16).  The cache must be bf16."""
+        block's output [tokens, out.n] (bf16).  The cache must be bf16.
+        With a stream that is not the current one the block runs there, after
+        what the current stream holds, on memory of that stream; the caller
+        has to order what reads the result after it."""
+        import torch
+        caller = torch.cuda.current_stream(self.ctx.device)
+        if stream is None:
+            return self._run(x, batch, caller)
+        if not isinstance(stream, torch.cuda.Stream):   # an address, as the other calls take it
+            stream = torch.cuda.ExternalStream(stream, self.ctx.device) if stream else \
+                torch.cuda.default_stream(self.ctx.device)
+        if stream == caller:
+            return self._run(x, batch, caller)
+        stream.wait_stream(caller)
+        with torch.cuda.stream(stream):
+            y = self._run(x, batch, stream)
+        # freed, these go back to their streams' memory only once both are through with them
+        for t in (x, *batch.tensors):
+            t.record_stream(stream)
+        y.record_stream(caller)
+        return y
+
+    def _run(self, x, batch, stream):
+        """The block on `stream`, which is the current one of the context's device."""
         row = tcc.qlinear(self.ctx, self.qkv, x, stream=stream)
         heads = row.view(x.shape[0], self.n_heads + 2 * self.n_kv, self.dim)
         q, k, v = heads.split((self.n_heads, self.n_kv, self.n_kv), 1)
