@@ -89,12 +89,17 @@ class AttentionBlock:
         self.window = window
 
     def __call__(self, x, batch: tcc.PagedBatch, stream=None):
-        """x: bf16 [tokens, hidden] of the step's new tokens; returns the
-        block's output [tokens, out.n] (bf16).  The cache must be bf16.
+        """x: contiguous bf16 [tokens, hidden] of the step's new tokens; returns
+        the block's output [tokens, out.n] (bf16).  The cache must be bf16.
         With a stream that is not the current one the block runs there, after
         what the current stream holds, on memory of that stream; the caller
         has to order what reads the result after it."""
         import torch
+        # (the projection takes its rows at their address, whatever they are)
+        if x.dtype is not torch.bfloat16 or x.dim() != 2 or x.shape[1] != self.qkv.k or not x.is_contiguous():
+            raise tcc.BackendError(f"x must be a contiguous bf16 tensor [tokens, {self.qkv.k}]")
+        if x.get_device() != self.ctx.device:
+            raise tcc.BackendError("x must be on the context's device")
         caller = torch.cuda.current_stream(self.ctx.device)
         if stream is None:
             return self._run(x, batch, caller)
