@@ -54,17 +54,33 @@ class PagePool:
         return [r + [-1] * (width - len(r)) for r in rows]
 
     def step(self, requests, new, device):
-        """Grows each request by its new tokens; the PagedBatch of the step."""
+        """Grows each request by its new tokens; the PagedBatch of the step.
+        A step that fails changes nothing."""
         import torch
-        lengths = [self.grow(r, n) for r, n in zip(requests, new)]
-        offsets = [0]
-        for n in new:
-            offsets.append(offsets[-1] + n)
+        requests, new = list(requests), list(new)
+        if len(requests) != len(new):
+            raise ValueError(f"{len(requests)} requests, new tokens of {len(new)}")
+        if not requests:
+            raise ValueError("a step needs a request")
 
         def ints(v):
             return torch.tensor(v, dtype=torch.int32, device=device)
-        return tcc.PagedBatch(ints(offsets), ints(lengths), ints(self.table(requests)), max(new, default=0),
-                              max(lengths, default=0))
+        lengths, offsets, before = [], [0], []
+        try:
+            for r, n in zip(requests, new):
+                pages, length = self._pages.get(r), self._length.get(r)
+                lengths.append(self.grow(r, n))
+                before.append((r, pages, length))
+                offsets.append(offsets[-1] + n)
+            return tcc.PagedBatch(ints(offsets), ints(lengths), ints(self.table(requests)), max(new), max(lengths))
+        except BaseException:
+            for r, pages, length in reversed(before):
+                self._free.extend(reversed(self._pages[r][len(pages or []):]))
+                if pages is None:
+                    del self._pages[r], self._length[r]
+                else:
+                    self._pages[r], self._length[r] = pages, length
+            raise
 
 
 class AttentionBlock:
