@@ -521,9 +521,10 @@ typedef struct tc_paged_cache {
  * is the page of its tokens j * page_size onward.  A request of length 0 (an
  * unused place of a fixed-size batch) caches and attends nothing.  Tokens from
  * new_offsets[n_seq] on belong to no request and are left alone.  max_new and
- * max_length bound the values in device memory (a request beyond them sets
- * TC_STATUS_GEOMETRY and is treated as having length 0, with no row past
- * max_new written); the launch is sized by them. */
+ * max_length bound the values in device memory; the launch is sized by them.
+ * A request beyond them, or with fewer cached tokens than new ones but not 0,
+ * sets TC_STATUS_GEOMETRY and is treated as having length 0, with no row past
+ * max_new written. */
 typedef struct tc_paged_batch {
     const int32_t *new_offsets;  /* [n_seq + 1] */
     const int32_t *lengths;      /* [n_seq] */

@@ -45,3 +45,64 @@ def test_a_weight_is_the_norms(ctx, dtype, layout):
         kept.append([y] + cache)
     assert all(torch.equal(a, b) for a, b in zip(*kept))
     assert ctx.status() == 0
+
+
+def _sentinels(ctx, lens, seen_lens, max_new, max_length, hq, hk, dim, dtype, seed):
+    """Attention and append of requests `lens` into outputs filled with 7,
+    bounded by max_new and max_length; (attention's out, lse, its reference
+    over seen_lens, append's q_out, cache before, cache after, status bits)."""
+    from turbocider_b200 import cuda as tcc
+    g = ac.gen(seed)
+    k, v, table, ks, vs = ac.paged([(0, max(n, 1)) for _, n in lens], 16, hk, dim, dtype, g, fill=0.0)
+    offsets, lengths = ac.offsets_of(lens)
+    tokens = int(offsets[-1])
+    q = ac.normal(g, (tokens, hq, dim), dtype)
+    batch = tcc.PagedBatch(offsets, lengths, table, max_new, max_length)
+    out = torch.full_like(q, 7.0)
+    _, lse = tcc.paged_attention(ctx, tcc.PagedCache(k, v), batch, q, out=out, return_lse=True)
+    bits = ctx.status()
+    want = ac.attention_ref(q, seen_lens, ks, vs, dim ** -0.5, True, 0)
+    turned = torch.full_like(q, 7.0)
+    k2, v2 = k.clone(), v.clone()
+    nk, nv = (ac.normal(g, (tokens, hk, dim), dtype) for _ in range(2))
+    tcc.kv_append(ctx, tcc.PagedCache(k2, v2), batch, nk, nv, q=q, q_out=turned)
+    assert ctx.status() == bits
+    return tcc, bits, q, out, want, turned, (k, v), (k2, v2), (nk, nv), table
+
+
+@pytest.mark.parametrize("dim,hq,hk", [(128, 8, 2), (64, 4, 4), (256, 2, 1)])
+@pytest.mark.parametrize("new,most,length", [(3, 1, 30), (5, 4, 5), (200, 100, 300), (130, 129, 130)])
+def test_a_request_past_max_new_is_cut(ctx, dim, hq, hk, new, most, length):
+    """It counts as one of length 0, reported, and its rows past max_new are
+    left alone; the other request is served."""
+    lens = [(new, length), (1, 20)]
+    tcc, bits, q, out, (want, _, tol, _), turned, old, fresh, (nk, nv), table = _sentinels(
+        ctx, lens, [(new, 0), (1, 20)], most, max(length, 20), hq, hk, dim, BF, seed=new)
+    assert bits == tcc.STATUS_GEOMETRY
+    assert bool((out[most:new] == 7).all()) and float(out[:most].abs().max()) == 0.0
+    ac.close(out[new:], want[new:], tol[new:])
+    assert bool((turned[most:new] == 7).all()) and torch.equal(turned[:most], q[:most])
+    assert torch.equal(turned[new:], q[new:])
+    page = int(table[1, 1])
+    for a, b, x in zip(old, fresh, (nk, nv)):
+        assert torch.equal(b[page, :, 3], x[new])
+        a[page, :, 3] = b[page, :, 3]
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dim,hq,hk", [(128, 8, 2), (64, 4, 4), (256, 2, 1)])
+@pytest.mark.parametrize("new,length", [(2, 1), (7, 3), (200, 199), (300, 40)])
+def test_a_request_shorter_than_its_new_tokens_is_impossible(ctx, dim, hq, hk, new, length):
+    """Lengths count the new tokens: less than them, but not 0, is reported and
+    treated as length 0."""
+    lens = [(new, length), (1, 20)]
+    tcc, bits, q, out, (want, _, tol, _), turned, old, fresh, (nk, nv), table = _sentinels(
+        ctx, lens, [(new, 0), (1, 20)], new, max(length, 20), hq, hk, dim, HF, seed=new)
+    assert bits == tcc.STATUS_GEOMETRY
+    assert float(out[:new].abs().max()) == 0.0
+    ac.close(out[new:], want[new:], tol[new:])
+    page = int(table[1, 1])
+    for a, b, x in zip(old, fresh, (nk, nv)):
+        assert torch.equal(b[page, :, 3], x[new])
+        a[page, :, 3] = b[page, :, 3]
+        assert torch.equal(a, b)

@@ -36,8 +36,9 @@ struct Request {
 };
 
 #ifdef __CUDACC__
-// A request with its values checked: rows inside q, a length that its row of
-// the page table covers, nothing past the bounds the launch was sized by.
+// A request with its values checked: rows inside q, a length that covers its
+// new tokens (0: an unused place) and that its row of the page table covers,
+// nothing past the bounds the launch was sized by.
 __device__ __forceinline__ Request check_request(const BatchView &bt, uint32_t page_shift, int32_t first, int32_t end,
                                                  int32_t length, uint32_t *status) {
     Request r{first, end - first, length};
@@ -46,9 +47,10 @@ __device__ __forceinline__ Request check_request(const BatchView &bt, uint32_t p
         return Request{0, 0, 0};
     }
     if (length < 0 || (uint32_t)length > bt.max_length || (uint32_t)r.n_new > bt.max_new ||
-        ((uint64_t)bt.table_width << page_shift) < (uint64_t)length) {
+        ((uint64_t)bt.table_width << page_shift) < (uint64_t)length || (length < r.n_new && length > 0)) {
         atomicOr(status, kStatusGeometry);
         r.length = 0;
+        r.n_new = min(r.n_new, (int32_t)bt.max_new);   // rows past it are nobody's
     }
     return r;
 }
