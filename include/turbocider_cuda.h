@@ -443,7 +443,8 @@ int tc_gguf_validate_split(const tc_gguf *const *shards, uint32_t n);
  * are device pointers; strides count elements; sums, norms, angles and the
  * softmax are fp32 or wider and every result is rounded once to its type.
  * Indices read from device memory (offsets, lengths, page numbers) are
- * checked there: an impossible one sets TC_STATUS_GEOMETRY and is skipped.
+ * checked there: an impossible one sets TC_STATUS_GEOMETRY and is skipped; the
+ * keys and values of an impossible page count as zeros.
  */
 
 /* Heads of one projection, as a [n_tokens][n_heads][head_dim] view.  `weight`

@@ -106,3 +106,26 @@ def test_a_request_shorter_than_its_new_tokens_is_impossible(ctx, dim, hq, hk, n
         assert torch.equal(b[page, :, 3], x[new])
         a[page, :, 3] = b[page, :, 3]
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("bad", [-1, -77, 10 ** 6, 2 ** 31 - 1])
+@pytest.mark.parametrize("dim,page", [(64, 8), (128, 16), (128, 256), (256, 32), (80, 64)])
+@pytest.mark.parametrize("new", [1, 5, 150])
+def test_a_page_outside_the_cache_reads_as_zeros(ctx, new, dim, page, bad):
+    """An impossible page number is reported, and no other page's tokens stand
+    in for its own."""
+    from turbocider_b200 import cuda as tcc
+    g = ac.gen(new + page)
+    lens = [(new, 700), (new, 300)]
+    k, v, table, ks, vs = ac.paged(lens, page, 2, dim, BF, g, fill=50.0)
+    first = int((table == 0).nonzero()[0, 0]) if bool((table == 0).any()) else -1   # whose tokens page 0 holds
+    which = 0 if first == 1 else 1
+    table[which, 1] = bad
+    for d in (ks, vs):
+        d[which][page:2 * page] = 0
+    offsets, lengths = ac.offsets_of(lens)
+    q = ac.normal(g, (2 * new, 4, dim), BF)
+    y = tcc.paged_attention(ctx, tcc.PagedCache(k, v), tcc.PagedBatch(offsets, lengths, table, new, 700), q)
+    assert ctx.status() == tcc.STATUS_GEOMETRY
+    want, _, tol, _ = ac.attention_ref(q, lens, ks, vs, dim ** -0.5, True, 0)
+    ac.close(y, want, tol)

@@ -385,7 +385,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int32_t pos = j * kChunkKeys + (int32_t)(piece * box);
             const bool on = pos < key_end;
             int32_t page = 0;
-            if (on) page = max(load_page(p.batch, p.n_pages, w.b, (uint32_t)pos >> p.page_shift, p.status), 0);
+            // (an impossible page is -1: a box outside the cache arrives as zeros)
+            if (on) page = load_page(p.batch, p.n_pages, w.b, (uint32_t)pos >> p.page_shift, p.status);
             const int token = (int)((uint32_t)pos & ((1u << p.page_shift) - 1));
             const uint32_t n_on = min(pieces, (uint32_t)(key_end - j * kChunkKeys + (int32_t)box - 1) / box);
 #pragma unroll 1

@@ -245,7 +245,8 @@ __global__ void __launch_bounds__(kWarps * 32)
         __syncwarp();
         if (box_piece < pieces) {
             const uint32_t pos = (uint32_t)key + box_piece * box;
-            const int page = max(pages[(pos >> p.page_shift) - ((uint32_t)begin >> p.page_shift)], 0);
+            // (an impossible page is -1: a box outside the cache arrives as zeros)
+            const int page = pages[(pos >> p.page_shift) - ((uint32_t)begin >> p.page_shift)];
             tma_load_4d(ring + st * L::stage + (lane & 1) * L::kv_bytes + box_half * (kKeys * 128) + box_piece * box * 128,
                         lane & 1 ? &vmap : &kmap, bar, (int)box_half * 64, (int)(pos & ((1u << p.page_shift) - 1)),
                         (int)h, page);
