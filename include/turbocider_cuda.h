@@ -548,6 +548,8 @@ int tc_cuda_kv_append(tc_cuda_ctx *ctx, const tc_paged_cache *cache, const tc_pa
  * its request's cache with
  *   causal:  j <= p, and j > p - window  where window > 0;
  *   else:    all,    and |j - p| < window where window > 0.
+ * Pages that end at or before the first position seen by any new token of a
+ * request are not looked up (a sliding window may have given them back).
  * A row that sees nothing gives zeros (lse -inf).  q and out are
  * [n_tokens][n_heads][head_dim] of the cache's dtype; lse (NULL: none) is f32
  * [n_tokens][n_heads], the natural log of the sum of exp(scale q k).  A NaN or

@@ -129,3 +129,27 @@ def test_a_page_outside_the_cache_reads_as_zeros(ctx, new, dim, page, bad):
     assert ctx.status() == tcc.STATUS_GEOMETRY
     want, _, tol, _ = ac.attention_ref(q, lens, ks, vs, dim ** -0.5, True, 0)
     ac.close(y, want, tol)
+
+
+@pytest.mark.parametrize("dim,hq,hk", [(64, 4, 2), (128, 8, 2), (256, 2, 2)])
+@pytest.mark.parametrize("page", [8, 16, 64, 128, 512])
+@pytest.mark.parametrize("new,window", [(1, 1), (1, 300), (5, 33), (40, 1000), (150, 7), (300, 520)])
+def test_pages_behind_a_window_may_be_given_back(ctx, dim, hq, hk, page, new, window):
+    """Pages that end before the first position that any new token sees are
+    neither looked up nor read."""
+    from turbocider_b200 import cuda as tcc
+    g = ac.gen(page + window)
+    lens = [(new, n) for n in (new, 1500, 2047, 4100)]
+    k, v, table, ks, vs = ac.paged(lens, page, hk, dim, BF, g)
+    for b, (_, n) in enumerate(lens):
+        gone = max(n - new - window + 1, 0) // page
+        for d in (k, v):
+            d[table[b, :gone].long()] = float("nan")
+        table[b, :gone] = -1
+    offsets, lengths = ac.offsets_of(lens)
+    q = ac.normal(g, (new * len(lens), hq, dim), BF)
+    y = tcc.paged_attention(ctx, tcc.PagedCache(k, v), tcc.PagedBatch(offsets, lengths, table, new, 4100), q,
+                            window=window)
+    assert ctx.status() == 0
+    want, _, tol, _ = ac.attention_ref(q, lens, ks, vs, dim ** -0.5, True, window)
+    ac.close(y, want, tol)

@@ -377,18 +377,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         // ---------------------------------------------------- TMA producer
         const uint32_t box = min((uint32_t)kChunkKeys, 1u << p.page_shift), pieces = kChunkKeys / box;
         const uint32_t piece = lane % pieces, half0 = lane / pieces;   // lanes: 32 / pieces halves at a time
-        const int32_t key_end = w.seen_hi;
+        const int32_t key_first = w.seen_lo, key_end = w.seen_hi;
         uint32_t st = 0, ph = 0, issued = 0;
         bool ok = true;
         for (int32_t j = w.begin; j < w.end; ++j) {
-            // this lane's page piece of the step
+            // this lane's page piece of the step (pages behind the first key seen may
+            // have been given back)
             const int32_t pos = j * kChunkKeys + (int32_t)(piece * box);
-            const bool on = pos < key_end;
+            const bool on = pos < key_end && pos + (int32_t)box > key_first;
             int32_t page = 0;
             // (an impossible page is -1: a box outside the cache arrives as zeros)
             if (on) page = load_page(p.batch, p.n_pages, w.b, (uint32_t)pos >> p.page_shift, p.status);
             const int token = (int)((uint32_t)pos & ((1u << p.page_shift) - 1));
-            const uint32_t n_on = min(pieces, (uint32_t)(key_end - j * kChunkKeys + (int32_t)box - 1) / box);
+            const uint32_t n_on = __popc(__ballot_sync(0xffffffffu, on && half0 == 0));
 #pragma unroll 1
             for (int kv = 0; kv < 2; ++kv) {
                 if (!(ok = wait(kv_empty(st), ph ^ 1))) break;

@@ -220,11 +220,12 @@ __global__ void __launch_bounds__(kWarps * 32)
     }
     const int32_t begin = base + (int32_t)(split * p.chunk), end = hi > lo ? min(hi, begin + (int32_t)p.chunk) : begin;
 
-    // ---- page numbers of the chunk
+    // ---- page numbers of the chunk, from the one with the first key seen on
+    // (earlier ones may have been given back)
     int32_t *pages = reinterpret_cast<int32_t *>(smem + L::page_off);
     if (end > begin) {
         const uint32_t j0 = (uint32_t)begin >> p.page_shift, j1 = (uint32_t)(end - 1) >> p.page_shift;
-        for (uint32_t j = j0 + threadIdx.x; j <= j1; j += kWarps * 32)
+        for (uint32_t j = ((uint32_t)max(begin, lo) >> p.page_shift) + threadIdx.x; j <= j1; j += kWarps * 32)
             pages[j - j0] = j == guess ? check_page(guessed, p.n_pages, p.status)
                                        : load_page(p.batch, p.n_pages, b, j, p.status);
     }
@@ -235,15 +236,17 @@ __global__ void __launch_bounds__(kWarps * 32)
     const int32_t steps = (end - begin + kKeys - 1) / kKeys;
     const uint32_t box = min((uint32_t)kKeys, 1u << p.page_shift);   // tokens of a TMA box
     // Loads of the warp's step i (16 keys from `key`), a lane for each box: K or
-    // V, half, and page piece, of the pieces that begin before the chunk's end.
+    // V, half, and page piece, of the pieces that begin before the chunk's end
+    // and end behind the first key seen.
     const uint32_t box_half = lane / 2 % L::halves, box_piece = lane / 2 / L::halves;
     auto issue = [&](int32_t i, uint32_t st) {
         const int32_t key = begin + i * kKeys;
         const uint32_t pieces = min((uint32_t)kKeys / box, (uint32_t)(end - key + (int32_t)box - 1) / box);
+        const uint32_t first = (uint32_t)max(lo - key, 0) / box;
         const uint32_t bar = bars + 8 * st;
-        if (lane == 0) bar_expect_tx(bar, pieces * box * DP * 4);
+        if (lane == 0) bar_expect_tx(bar, (pieces - first) * box * DP * 4);
         __syncwarp();
-        if (box_piece < pieces) {
+        if (box_piece >= first && box_piece < pieces) {
             const uint32_t pos = (uint32_t)key + box_piece * box;
             // (an impossible page is -1: a box outside the cache arrives as zeros)
             const int page = pages[(pos >> p.page_shift) - ((uint32_t)begin >> p.page_shift)];
