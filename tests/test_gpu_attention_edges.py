@@ -153,3 +153,70 @@ def test_pages_behind_a_window_may_be_given_back(ctx, dim, hq, hk, page, new, wi
     assert ctx.status() == 0
     want, _, tol, _ = ac.attention_ref(q, lens, ks, vs, dim ** -0.5, True, window)
     ac.close(y, want, tol)
+
+
+def test_more_tiles_than_a_grid_dimension(ctx):
+    """Heads of 256: 4100 requests of up to 257 rows make 69700 tiles."""
+    from turbocider_b200 import cuda as tcc
+    g, dim, page = ac.gen(41), 256, 16
+    lens = [(1, 1 + i % 16) for i in range(4100)]
+    lens[1234] = (257, 300)
+    k, v, table, ks, vs = ac.paged(lens, page, 1, dim, BF, g)
+    offsets, lengths = ac.offsets_of(lens)
+    q = ac.normal(g, (int(offsets[-1]), 1, dim), BF)
+    y, lse = tcc.paged_attention(ctx, tcc.PagedCache(k, v), tcc.PagedBatch(offsets, lengths, table, 257, 300), q,
+                                 return_lse=True)
+    assert ctx.status() == 0
+    want, wlse, tol, tol_lse = ac.attention_ref(q, lens, ks, vs, dim ** -0.5, True, 0)
+    ac.close(y, want, tol)
+    ac.close(lse, wlse, tol_lse)
+
+
+def test_more_requests_than_a_grid_dimension(ctx):
+    """70000 requests of one token over the same two pages."""
+    from turbocider_b200 import cuda as tcc
+    g, n, dim = ac.gen(42), 70000, 64
+    k, v, table, ks, vs = ac.paged([(1, 13)], 8, 2, dim, HF, g)
+    q = ac.normal(g, (n, 4, dim), HF)
+    y = tcc.paged_attention(ctx, tcc.PagedCache(k, v),
+                            tcc.PagedBatch(torch.arange(n + 1, dtype=torch.int32, device="cuda"),
+                                           torch.full((n,), 13, dtype=torch.int32, device="cuda"),
+                                           table.expand(n, -1).contiguous(), 1, 13), q)
+    assert ctx.status() == 0
+    want, _, tol, _ = ac.attention_ref(q, [(n, 13)], ks, vs, dim ** -0.5, False, 0)   # every row sees all 13
+    ac.close(y, want, tol)
+
+
+@pytest.mark.parametrize("dim,n,hk,group", [(256, 700, 8, 16), (128, 600, 8, 32)])
+def test_partial_results_past_the_workspaces_bound(ctx, dim, n, hk, group):
+    """Requests whose partial results together pass the bound of the workspace
+    (all over the same pages, so that the cache stays small)."""
+    from turbocider_b200 import cuda as tcc
+    g, length = ac.gen(43), 4000
+    k, v, table, ks, vs = ac.paged([(1, length)], 64, hk, dim, BF, g)
+    q = ac.normal(g, (n, hk * group, dim), BF)
+    args = (torch.arange(n + 1, dtype=torch.int32, device="cuda"),
+            torch.full((n,), length, dtype=torch.int32, device="cuda"), table.expand(n, -1).contiguous(), 1, length)
+    y = tcc.paged_attention(ctx, tcc.PagedCache(k, v), tcc.PagedBatch(*args), q)
+    again = tcc.paged_attention(ctx, tcc.PagedCache(k, v), tcc.PagedBatch(*args), q)
+    assert ctx.status() == 0 and torch.equal(y, again)
+    want, _, tol, _ = ac.attention_ref(q, [(n, length)], ks, vs, dim ** -0.5, False, 0)   # every row sees all of them
+    ac.close(y, want, tol)
+
+
+@pytest.mark.parametrize("length", [150001, 140000])
+def test_very_many_shares(ctx, length):
+    """64 rows of 64 over so long a cache that the statistics of its shares do
+    not fit the memory that the last CTA joins them in."""
+    from turbocider_b200 import cuda as tcc
+    g = ac.gen(45)
+    lens = [(4, length)]
+    k, v, table, ks, vs = ac.paged(lens, 256, 1, 64, BF, g)
+    offsets, lengths = ac.offsets_of(lens)
+    q = ac.normal(g, (4, 16, 64), BF)
+    y, lse = tcc.paged_attention(ctx, tcc.PagedCache(k, v), tcc.PagedBatch(offsets, lengths, table, 4, length), q,
+                                 return_lse=True)
+    assert ctx.status() == 0
+    want, wlse, tol, tol_lse = ac.attention_ref(q, lens, ks, vs, 64 ** -0.5, True, 0)
+    ac.close(y, want, tol)
+    ac.close(lse, wlse, tol_lse)

@@ -18,6 +18,7 @@ struct AttnParams {
     uint32_t *status;
     // row tiles of a request and chunks of its cache
     uint32_t row_tiles, chunk, splits;
+    uint32_t first_unit;         // few rows: request and row tile of the launch's first CTAs
     // partial results: [tile][split][ws_rows] of (maximum, sum), then of the
     // unnormalised outputs from float ws_ml on
     uint32_t ws_rows;

@@ -183,7 +183,8 @@ __global__ void __launch_bounds__(kWarps * 32)
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const uint32_t split = blockIdx.x, h = blockIdx.y, b = blockIdx.z / p.row_tiles, rt = blockIdx.z % p.row_tiles;
+    const uint32_t split = blockIdx.x, h = blockIdx.y, unit = p.first_unit + blockIdx.z;
+    const uint32_t b = unit / p.row_tiles, rt = unit % p.row_tiles;
     volatile uint32_t *abort_flag = reinterpret_cast<uint32_t *>(smem + L::misc_off);
     uint32_t *last_flag = reinterpret_cast<uint32_t *>(smem + L::misc_off) + 1;
     const uint32_t bars = su32(smem + L::bar_off) + warp * L::stages * 8;
@@ -564,6 +565,10 @@ bool encode_cache(CUtensorMap *map, const uint16_t *base, const CacheView &c, ui
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Bytes of partial results that one launch asks the workspace for, at most
+// (where one unit of work needs no more).
+constexpr uint64_t kWorkspaceMost = 256u << 20;
+
 // Grows the context's split workspace; the counters start at zero and every
 // complete kernel leaves them so.
 int ensure_split(tc_cuda_ctx *ctx, size_t floats, size_t counters, cudaStream_t s) {
@@ -690,7 +695,7 @@ int attend(tc_cuda_ctx *ctx, const tc_paged_cache *cache, const tc_paged_batch *
     }
     p.row_tiles = (uint32_t)((rows_most + 16 * mt - 1) / (16 * mt));
     const uint64_t units = (uint64_t)p.batch.n_seq * p.row_tiles;
-    if (units > 65535) return fail("too many tokens or requests");
+    if (units > 0x7fffffffu) return fail("too many tokens or requests");
     const uint32_t keys = step_keys((int)dp, (int)mt);
     span += keys;   // the first key is rounded down to a step
     // Chunk of the cache per CTA: the least of (rounds of CTAs over the GPU's
@@ -711,10 +716,15 @@ int attend(tc_cuda_ctx *ctx, const tc_paged_cache *cache, const tc_paged_batch *
     p.chunk = (uint32_t)chunk;
     p.splits = (uint32_t)((span + chunk - 1) / chunk);
     p.ws_rows = (uint32_t)std::min<uint64_t>(rows_most, 16 * mt);
+    // Units of a launch: a dimension of the grid, and no more than their partial
+    // results fit kWorkspaceMost bytes (at 16 KB or so a CTA that leaves tens of
+    // rounds over the GPU; launches on a stream take turns with the workspace).
+    uint64_t each = std::min<uint64_t>(units, 65535);
     if (p.splits > 1) {
-        const uint64_t parts = units * c.n_heads * p.splits * p.ws_rows;
-        p.ws_ml = (parts * 2 + 3) / 4 * 4;
-        if (ensure_split(ctx, p.ws_ml + parts * dp, units * c.n_heads, s)) return TC_CUDA_FAIL;
+        const uint64_t parts = (uint64_t)c.n_heads * p.splits * p.ws_rows;   // of a unit
+        each = std::max<uint64_t>(std::min(each, kWorkspaceMost / (parts * (dp + 2) * sizeof(float))), 1);
+        p.ws_ml = (each * parts * 2 + 3) / 4 * 4;
+        if (ensure_split(ctx, p.ws_ml + each * parts * dp, each * c.n_heads, s)) return TC_CUDA_FAIL;
         p.ws = ctx->attn_ws;
         p.counters = ctx->attn_counters;
     }
@@ -722,16 +732,19 @@ int attend(tc_cuda_ctx *ctx, const tc_paged_cache *cache, const tc_paged_batch *
     const uint32_t box = c.page_size < keys ? c.page_size : keys;
     if (!encode_cache(&km, c.k, c, box, bf16) || !encode_cache(&vm, c.v, c, box, bf16))
         return fail("the cache cannot be described to TMA");
-    const dim3 grid(p.splits, c.n_heads, (uint32_t)units);
-    cudaError_t e;
-    if (dp == 64)
-        e = mt == 1   ? launch_few_t<64, 1>(km, vm, p, bf16, grid, s)
-            : mt == 2 ? launch_few_t<64, 2>(km, vm, p, bf16, grid, s)
-                      : launch_few_t<64, 4>(km, vm, p, bf16, grid, s);
-    else if (dp == 128)
-        e = mt == 1 ? launch_few_t<128, 1>(km, vm, p, bf16, grid, s) : launch_few_t<128, 2>(km, vm, p, bf16, grid, s);
-    else
-        e = launch_few_t<256, 1>(km, vm, p, bf16, grid, s);
+    cudaError_t e = cudaSuccess;
+    for (uint64_t first = 0; first < units && e == cudaSuccess; first += each) {
+        p.first_unit = (uint32_t)first;
+        const dim3 grid(p.splits, c.n_heads, (uint32_t)std::min(each, units - first));
+        if (dp == 64)
+            e = mt == 1   ? launch_few_t<64, 1>(km, vm, p, bf16, grid, s)
+                : mt == 2 ? launch_few_t<64, 2>(km, vm, p, bf16, grid, s)
+                          : launch_few_t<64, 4>(km, vm, p, bf16, grid, s);
+        else if (dp == 128)
+            e = mt == 1 ? launch_few_t<128, 1>(km, vm, p, bf16, grid, s) : launch_few_t<128, 2>(km, vm, p, bf16, grid, s);
+        else
+            e = launch_few_t<256, 1>(km, vm, p, bf16, grid, s);
+    }
     return e == cudaSuccess ? ok() : cuda_fail("paged attention launch", e);
 }
 
