@@ -204,6 +204,21 @@ def test_partial_results_past_the_workspaces_bound(ctx, dim, n, hk, group):
     ac.close(y, want, tol)
 
 
+def test_a_loose_bound_on_the_lengths(ctx):
+    """max_length far past what the page table covers asks for no more
+    workspace than the table can mean."""
+    from turbocider_b200 import cuda as tcc
+    g = ac.gen(44)
+    lens = [(1, 300 - i) for i in range(64)]
+    k, v, table, ks, vs = ac.paged(lens, 16, 8, 128, BF, g)
+    offsets, lengths = ac.offsets_of(lens)
+    q = ac.normal(g, (64, 32, 128), BF)
+    y = tcc.paged_attention(ctx, tcc.PagedCache(k, v), tcc.PagedBatch(offsets, lengths, table, 1, 2 ** 30), q)
+    assert ctx.status() == 0
+    want, _, tol, _ = ac.attention_ref(q, lens, ks, vs, 128 ** -0.5, True, 0)
+    ac.close(y, want, tol)
+
+
 @pytest.mark.parametrize("length", [150001, 140000])
 def test_very_many_shares(ctx, length):
     """64 rows of 64 over so long a cache that the statistics of its shares do

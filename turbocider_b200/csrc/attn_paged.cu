@@ -639,8 +639,9 @@ int attend(tc_cuda_ctx *ctx, const tc_paged_cache *cache, const tc_paged_batch *
     p.out_quads = !(reinterpret_cast<uintptr_t>(a->out) % 8) && !(a->ld_out_token % 4) && !(a->ld_out_head % 4);
     const bool bf16 = cache->dtype == TC_DTYPE_BF16;
 
-    // longest span of keys one tile of rows sees
-    uint64_t span = p.batch.max_length;
+    // longest span of keys one tile of rows sees (requests that their row of the
+    // page table does not cover are not served)
+    uint64_t span = std::min<uint64_t>(p.batch.max_length, (uint64_t)p.batch.table_width << p.page_shift);
     if (p.window) {
         const uint64_t reach = (uint64_t)p.window * (p.causal ? 1 : 2) + p.batch.max_new;
         if (reach < span) span = reach;
