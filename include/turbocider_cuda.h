@@ -571,6 +571,21 @@ typedef struct tc_attention {
 int tc_cuda_paged_attention(tc_cuda_ctx *ctx, const tc_paged_cache *cache, const tc_paged_batch *batch,
                             const tc_attention *attention, void *stream);
 
+/* How tc_cuda_paged_attention divides a call of these sizes on a GPU of
+ * sm_count SMs.  Of `batch` the sizes alone are read.  No launch and no GPU; for
+ * tests and for sizing work. */
+typedef struct tc_attention_plan {
+    uint32_t many_rows;          /* 1: the tensor-core kernel of whole blocks of rows */
+    uint32_t rows;               /* of a CTA */
+    uint32_t ctas_per_sm;
+    uint32_t share_keys, shares; /* keys of a CTA, CTAs that the longest span is split over */
+    uint32_t launches;
+    uint64_t workspace_bytes;    /* of the context's workspace, 0: none */
+} tc_attention_plan;
+int tc_paged_attention_plan(uint32_t sm_count, uint32_t n_heads, uint32_t cache_heads, uint32_t head_dim,
+                            uint32_t page_size, const tc_paged_batch *batch, int32_t causal, int32_t window,
+                            tc_attention_plan *plan);
+
 /* Host-side GGUF K-quant quantiser (not in the reference, which ships no
  * encoder): quantise a row-major fp32 [rows, cols] matrix (cols % 256 == 0) to
  * raw GGUF blocks of `ggml_type` (Q4_K or Q6_K) using `threads` CPU threads.

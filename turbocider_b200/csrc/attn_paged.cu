@@ -43,6 +43,9 @@ namespace {
 constexpr int step_keys(int dp, int mt) { return dp == 64 && mt <= 2 ? 32 : 16; }
 constexpr int kWarps = 4;
 constexpr uint32_t kMaxChunk = 1024;
+// CTAs that an SM has room for: by the rings for 16 rows (heads of 256 need 128 KB
+// for two stages), by the registers of 32 and 64 rows.
+constexpr int ctas_per_sm(int dp, int mt) { return dp == 256 ? 1 : mt == 1 ? 3 : 2; }
 
 // Rows of a CTA: MT mma tiles of 16.
 template <int DP, int MT>
@@ -52,8 +55,9 @@ struct FewLayout {
     static constexpr int keys = step_keys(DP, MT);
     static constexpr uint32_t kv_bytes = keys * DP * 2;       // K of a step; V follows
     static constexpr uint32_t stage = 2 * kv_bytes;
-    // 64 KB of rings: three CTAs per SM.  (Three stages and two CTAs kept as
-    // much in flight but took 265 us, not 245, for 1.5 GB of cache.)
+    // 64 KB of rings (128 for heads of 256).  (Three stages and two CTAs an SM kept
+    // as much in flight as two and three but took 265 us, not 245, for 1.5 GB of
+    // cache.)
     static constexpr int stages = DP == 64 && keys == 16 ? 4 : 2;
     static constexpr uint32_t ring = stages * stage;           // per warp
     static constexpr uint32_t q_off = kWarps * ring;           // queries: rows x DP, 16-byte pieces swizzled by row
@@ -62,6 +66,8 @@ struct FewLayout {
     static constexpr uint32_t ml_off = page_off + (kMaxChunk / 8 + 2) * 4;   // [warp][row][m, l]
     static constexpr uint32_t misc_off = ml_off + kWarps * rows * 8;
     static constexpr uint32_t bytes = misc_off + 16 + 1024;
+    static constexpr int places = ctas_per_sm(DP, MT);
+    static_assert(places * (bytes + 1024) <= 233472, "the CTAs of an SM share its memory");
     static_assert(kWarps * ring >= kWarps * rows * DP * 4, "the join reuses the rings");
     static constexpr uint32_t max_shares = kWarps * ring / (rows * 8);   // whose statistics fit there too
 };
@@ -175,7 +181,7 @@ __device__ __forceinline__ void join_shares(const AttnParams &p, const Request &
 }
 
 template <int DP, int MT, bool BF16>
-__global__ void __launch_bounds__(kWarps * 32)
+__global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(DP, MT))
     few_rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                     const __grid_constant__ AttnParams p) {
     using L = FewLayout<DP, MT>;
@@ -597,6 +603,99 @@ int ensure_split(tc_cuda_ctx *ctx, size_t floats, size_t counters, cudaStream_t 
     return TC_CUDA_OK;
 }
 
+// How a call is divided over CTAs, by its sizes alone.
+struct AttnPlan {
+    bool many;                 // attn_chunk_sm100.cu's kernel, else this file's
+    uint32_t dp, mt;           // head_dim padded; mma tiles of a CTA (few rows)
+    uint32_t chunk, splits;    // keys of a share, shares
+    uint32_t n_blocks;         // many rows: upper bound of the blocks of rows
+    uint32_t row_tiles, ws_rows;
+    uint64_t units, each;      // few rows: requests x row tiles, of which a launch takes `each`
+    uint64_t ws_ml, ws_floats, counters;   // workspace (0: none)
+};
+
+const char *plan_attention(const BatchView &bt, uint32_t n_kv, uint64_t group, uint32_t head_dim, uint32_t page_shift,
+                           bool causal, int32_t window, uint32_t sm_count, AttnPlan &a) {
+    a = AttnPlan{};
+    // longest span of keys one tile of rows sees (requests that their row of the
+    // page table does not cover are not served)
+    uint64_t span = std::min<uint64_t>(bt.max_length, (uint64_t)bt.table_width << page_shift);
+    if (window) {
+        const uint64_t reach = (uint64_t)window * (causal ? 1 : 2) + bt.max_new;
+        if (reach < span) span = reach;
+    }
+    const uint64_t rows_most = group * bt.max_new;
+    // mma tiles of a CTA: all rows of a request in one CTA, so that K and V are
+    // read once, as far as the registers go.
+    const uint32_t dp = a.dp = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
+    const uint32_t mt = a.mt = rows_most <= 16 || dp == 256 ? 1 : rows_most <= 32 || dp == 128 ? 2 : 4;
+    a.many = rows_most > mt * 16 && head_dim <= 128;
+    if (a.many) {
+        const uint64_t rows = (uint64_t)bt.n_tokens * group;
+        a.n_blocks = (uint32_t)(rows / kChunkRows + bt.n_seq);
+        // Shares of the keys: as many CTAs as make the busiest SM's work least,
+        // in steps of 128 keys plus kCtaSteps for what a CTA does besides, one
+        // CTA per SM, and the time to join the shares (2 us and 0.5 us a share,
+        // in steps of 2 us); no share under kLeastSteps.
+        constexpr uint64_t kCtaSteps = 3, kLeastSteps = 2;
+        const uint64_t steps = (span + kChunkKeys - 1) / kChunkKeys + 1;
+        const uint64_t blocks = std::max<uint64_t>((rows + kChunkRows - 1) / kChunkRows, bt.n_seq);
+        uint64_t best = ~0ull, share = steps;
+        for (uint64_t n = 1; n <= kChunkShares && (n == 1 || steps / n >= kLeastSteps); ++n) {
+            const uint64_t each = (steps + n - 1) / n, real = (steps + each - 1) / each;
+            const uint64_t waves = (blocks * n_kv * real + sm_count - 1) / sm_count;
+            const uint64_t cost = 4 * waves * (each + kCtaSteps) + (real > 1 ? 4 + real : 0);
+            if (cost < best) {
+                best = cost;
+                share = each;
+            }
+        }
+        a.chunk = (uint32_t)(share * kChunkKeys);
+        a.splits = (uint32_t)((steps + share - 1) / share);
+        if ((uint64_t)a.n_blocks * n_kv * a.splits > 0x7fffffffu) return "too many tokens or requests";
+        if (a.splits > 1) {
+            const uint64_t parts = (uint64_t)a.n_blocks * n_kv * a.splits * kChunkRows;
+            a.ws_ml = parts * 2;
+            a.ws_floats = a.ws_ml + parts * dp;
+        }
+        return nullptr;
+    }
+    a.row_tiles = (uint32_t)((rows_most + 16 * mt - 1) / (16 * mt));
+    a.units = (uint64_t)bt.n_seq * a.row_tiles;
+    if (a.units > 0x7fffffffu) return "too many tokens or requests";
+    span += step_keys((int)dp, (int)mt);   // the first key is rounded down to a step
+    // Chunk of the cache per CTA: the least of (rounds of CTAs over the GPU's
+    // places) x (a chunk's time + what a CTA costs besides) + the time to join
+    // the shares, all in keys: about 100 KB for a CTA's start and end (7 us
+    // against 15 GB/s a place), 8 keys a share.  8 requests of 6000 keys of 64 by 28
+    // rows: 7 shares, one round, 29 us; 11 shares in two rounds 41 us.
+    const uint64_t places = (uint64_t)sm_count * ctas_per_sm((int)dp, (int)mt), cta_keys = 100 * 1024 / (4 * dp);
+    uint64_t chunk = kMaxChunk, best = ~0ull;
+    for (uint64_t c = kMaxChunk; c >= 64; c -= 64) {
+        const uint64_t n = (span + c - 1) / c, rounds = (a.units * n * n_kv + places - 1) / places;
+        const uint64_t cost = rounds * (c + cta_keys) + 8 * n;
+        if (cost < best) {
+            best = cost;
+            chunk = c;
+        }
+    }
+    a.chunk = (uint32_t)chunk;
+    a.splits = (uint32_t)((span + chunk - 1) / chunk);
+    a.ws_rows = (uint32_t)std::min<uint64_t>(rows_most, 16 * mt);
+    // Units of a launch: a dimension of the grid, and no more than their partial
+    // results fit kWorkspaceMost bytes (at 16 KB or so a CTA that leaves tens of
+    // rounds over the GPU; launches on a stream take turns with the workspace).
+    a.each = std::min<uint64_t>(a.units, 65535);
+    if (a.splits > 1) {
+        const uint64_t parts = (uint64_t)n_kv * a.splits * a.ws_rows;   // of a unit
+        a.each = std::max<uint64_t>(std::min(a.each, kWorkspaceMost / (parts * (dp + 2) * sizeof(float))), 1);
+        a.ws_ml = (a.each * parts * 2 + 3) / 4 * 4;
+        a.ws_floats = a.ws_ml + a.each * parts * dp;
+        a.counters = a.each * n_kv;
+    }
+    return nullptr;
+}
+
 int attend(tc_cuda_ctx *ctx, const tc_paged_cache *cache, const tc_paged_batch *batch, const tc_attention *a,
            cudaStream_t s) {
     CacheView c{};
@@ -639,104 +738,41 @@ int attend(tc_cuda_ctx *ctx, const tc_paged_cache *cache, const tc_paged_batch *
     p.out_quads = !(reinterpret_cast<uintptr_t>(a->out) % 8) && !(a->ld_out_token % 4) && !(a->ld_out_head % 4);
     const bool bf16 = cache->dtype == TC_DTYPE_BF16;
 
-    // longest span of keys one tile of rows sees (requests that their row of the
-    // page table does not cover are not served)
-    uint64_t span = std::min<uint64_t>(p.batch.max_length, (uint64_t)p.batch.table_width << p.page_shift);
-    if (p.window) {
-        const uint64_t reach = (uint64_t)p.window * (p.causal ? 1 : 2) + p.batch.max_new;
-        if (reach < span) span = reach;
-    }
+    AttnPlan plan;
+    if (const char *e = plan_attention(p.batch, c.n_heads, group, c.head_dim, c.page_shift, p.causal, p.window,
+                                       (uint32_t)ctx->sm_count, plan))
+        return fail(e);
+    p.chunk = plan.chunk;
+    p.splits = plan.splits;
+    p.n_blocks = plan.n_blocks;
+    p.row_tiles = plan.row_tiles;
+    p.ws_rows = plan.ws_rows;
+    p.ws_ml = plan.ws_ml;
     CurrentDevice guard(ctx->device);
-
-    const uint64_t rows_most = group * p.batch.max_new;
-    // mma tiles of a CTA: all rows of a request in one CTA, so that K and V are
-    // read once, as far as the registers go.
-    const uint32_t dp = c.head_dim <= 64 ? 64 : c.head_dim <= 128 ? 128 : 256;
-    const uint32_t mt = rows_most <= 16 || dp == 256 ? 1 : rows_most <= 32 || dp == 128 ? 2 : 4;
-    if (rows_most > mt * 16 && c.head_dim <= 128) {
-        const uint64_t rows = (uint64_t)p.batch.n_tokens * group;
-        p.n_blocks = (uint32_t)(rows / kChunkRows + p.batch.n_seq);
+    if (plan.ws_floats) {
+        if (ensure_split(ctx, plan.ws_floats, plan.counters, s)) return TC_CUDA_FAIL;
+        p.ws = ctx->attn_ws;
+        p.counters = ctx->attn_counters;
+    }
+    const uint32_t dp = plan.dp, mt = plan.mt;
+    const uint32_t keys = plan.many ? kChunkKeys : step_keys((int)dp, (int)mt);
+    CUtensorMap km, vm;
+    const uint32_t box = c.page_size < keys ? c.page_size : keys;
+    if (!encode_cache(&km, c.k, c, box, bf16) || !encode_cache(&vm, c.v, c, box, bf16))
+        return fail("the cache cannot be described to TMA");
+    if (plan.many) {
         const uint64_t out_bits = reinterpret_cast<uintptr_t>(a->out) | a->ld_out_token * 2 | a->ld_out_head * 2;
         p.out_wide = out_bits % 32 == 0 ? 32 : out_bits % 16 == 0 ? 16 : 0;
         p.negate_q = p.scale_log2 < 0.f;
         p.scale_log2 = std::fabs(p.scale_log2);
         if (p.scale_log2 < 1e-30f) p.scale_log2 = 1e-30f;   // 0 * -inf would lose the mask
-        // Shares of the keys: as many CTAs as make the busiest SM's work least,
-        // in steps of 128 keys plus kCtaSteps for what a CTA does besides, one
-        // CTA per SM, and the time to join the shares (2 us and 0.5 us a share,
-        // in steps of 2 us); no share under kLeastSteps.
-        constexpr uint64_t kCtaSteps = 3, kLeastSteps = 2;
-        const uint64_t steps = (span + kChunkKeys - 1) / kChunkKeys + 1;
-        const uint64_t blocks = std::max<uint64_t>((rows + kChunkRows - 1) / kChunkRows, p.batch.n_seq);
-        uint64_t best = ~0ull, share = steps;
-        for (uint64_t n = 1; n <= kChunkShares && (n == 1 || steps / n >= kLeastSteps); ++n) {
-            const uint64_t each = (steps + n - 1) / n, real = (steps + each - 1) / each;
-            const uint64_t waves = (blocks * c.n_heads * real + ctx->sm_count - 1) / ctx->sm_count;
-            const uint64_t cost = 4 * waves * (each + kCtaSteps) + (real > 1 ? 4 + real : 0);
-            if (cost < best) {
-                best = cost;
-                share = each;
-            }
-        }
-        p.chunk = (uint32_t)(share * kChunkKeys);
-        p.splits = (uint32_t)((steps + share - 1) / share);
-        if ((uint64_t)p.n_blocks * c.n_heads * p.splits > 0x7fffffffu) return fail("too many tokens or requests");
-        if (p.splits > 1) {
-            const uint64_t parts = (uint64_t)p.n_blocks * c.n_heads * p.splits * kChunkRows;
-            p.ws_ml = parts * 2;
-            if (ensure_split(ctx, p.ws_ml + parts * dp, 0, s)) return TC_CUDA_FAIL;
-            p.ws = ctx->attn_ws;
-        }
-        CUtensorMap km, vm;
-        const uint32_t box = c.page_size < kChunkKeys ? c.page_size : kChunkKeys;
-        if (!encode_cache(&km, c.k, c, box, bf16) || !encode_cache(&vm, c.v, c, box, bf16))
-            return fail("the cache cannot be described to TMA");
         const cudaError_t e = launch_chunk(km, vm, p, bf16, s);
         return e == cudaSuccess ? ok() : cuda_fail("paged attention launch", e);
     }
-    p.row_tiles = (uint32_t)((rows_most + 16 * mt - 1) / (16 * mt));
-    const uint64_t units = (uint64_t)p.batch.n_seq * p.row_tiles;
-    if (units > 0x7fffffffu) return fail("too many tokens or requests");
-    const uint32_t keys = step_keys((int)dp, (int)mt);
-    span += keys;   // the first key is rounded down to a step
-    // Chunk of the cache per CTA: the least of (rounds of CTAs over the GPU's
-    // places) x (a chunk's time + what a CTA costs besides) + the time to join
-    // the shares, all in keys: about 100 KB for a CTA's start and end (7 us
-    // against 15 GB/s a place), 8 keys a share.  23 requests of 2071 keys by 28
-    // rows: 3 shares, 17 us; with many short ones (11 shares) 41 us.
-    const uint64_t places = (uint64_t)ctx->sm_count * (mt == 1 || (dp == 64 && mt == 2) ? 3 : 2), cta_keys = 100 * 1024 / (4 * dp);
-    uint64_t chunk = kMaxChunk, best = ~0ull;
-    for (uint64_t c = kMaxChunk; c >= 64; c -= 64) {
-        const uint64_t n = (span + c - 1) / c, rounds = (units * n * p.n_kv + places - 1) / places;
-        const uint64_t cost = rounds * (c + cta_keys) + 8 * n;
-        if (cost < best) {
-            best = cost;
-            chunk = c;
-        }
-    }
-    p.chunk = (uint32_t)chunk;
-    p.splits = (uint32_t)((span + chunk - 1) / chunk);
-    p.ws_rows = (uint32_t)std::min<uint64_t>(rows_most, 16 * mt);
-    // Units of a launch: a dimension of the grid, and no more than their partial
-    // results fit kWorkspaceMost bytes (at 16 KB or so a CTA that leaves tens of
-    // rounds over the GPU; launches on a stream take turns with the workspace).
-    uint64_t each = std::min<uint64_t>(units, 65535);
-    if (p.splits > 1) {
-        const uint64_t parts = (uint64_t)c.n_heads * p.splits * p.ws_rows;   // of a unit
-        each = std::max<uint64_t>(std::min(each, kWorkspaceMost / (parts * (dp + 2) * sizeof(float))), 1);
-        p.ws_ml = (each * parts * 2 + 3) / 4 * 4;
-        if (ensure_split(ctx, p.ws_ml + each * parts * dp, each * c.n_heads, s)) return TC_CUDA_FAIL;
-        p.ws = ctx->attn_ws;
-        p.counters = ctx->attn_counters;
-    }
-    CUtensorMap km, vm;
-    const uint32_t box = c.page_size < keys ? c.page_size : keys;
-    if (!encode_cache(&km, c.k, c, box, bf16) || !encode_cache(&vm, c.v, c, box, bf16))
-        return fail("the cache cannot be described to TMA");
     cudaError_t e = cudaSuccess;
-    for (uint64_t first = 0; first < units && e == cudaSuccess; first += each) {
+    for (uint64_t first = 0; first < plan.units && e == cudaSuccess; first += plan.each) {
         p.first_unit = (uint32_t)first;
-        const dim3 grid(p.splits, c.n_heads, (uint32_t)std::min(each, units - first));
+        const dim3 grid(p.splits, c.n_heads, (uint32_t)std::min(plan.each, plan.units - first));
         if (dp == 64)
             e = mt == 1   ? launch_few_t<64, 1>(km, vm, p, bf16, grid, s)
                 : mt == 2 ? launch_few_t<64, 2>(km, vm, p, bf16, grid, s)
@@ -751,6 +787,39 @@ int attend(tc_cuda_ctx *ctx, const tc_paged_cache *cache, const tc_paged_batch *
 
 }  // namespace
 }  // namespace tc
+
+extern "C" int tc_paged_attention_plan(uint32_t sm_count, uint32_t n_heads, uint32_t cache_heads, uint32_t head_dim,
+                                       uint32_t page_size, const tc_paged_batch *batch, int32_t causal, int32_t window,
+                                       tc_attention_plan *plan) {
+    using namespace tc;
+    if (!batch || !plan) return fail("null argument");
+    if (!sm_count || !head_dim || head_dim % 8 || head_dim > 256 || !cache_heads || cache_heads > 65535 || !n_heads ||
+        n_heads % cache_heads || page_size < 8 || page_size > 65536 || (page_size & (page_size - 1)) || window < 0 ||
+        batch->max_length > (uint32_t)kMaxLength || !batch->n_seq || batch->n_seq > 0xffffffu || !batch->n_tokens ||
+        batch->n_tokens > 0x7fffffffu || !batch->max_new)
+        return fail("sizes that tc_cuda_paged_attention would not take");
+    BatchView bt{};
+    bt.n_seq = batch->n_seq;
+    bt.table_width = batch->table_width;
+    bt.n_tokens = batch->n_tokens;
+    bt.max_new = std::min(batch->max_new, batch->n_tokens);
+    bt.max_length = batch->max_length;
+    const uint64_t group = n_heads / cache_heads;
+    if (group * bt.max_new > 0x7fffffffu) return fail("too many heads");
+    AttnPlan a;
+    if (const char *e = plan_attention(bt, cache_heads, group, head_dim, (uint32_t)__builtin_ctz(page_size), causal != 0,
+                                       std::min(window, kMaxLength), sm_count, a))
+        return fail(e);
+    *plan = tc_attention_plan{};
+    plan->many_rows = a.many;
+    plan->rows = a.many ? kChunkRows : 16 * a.mt;
+    plan->ctas_per_sm = a.many ? 1 : (uint32_t)ctas_per_sm((int)a.dp, (int)a.mt);
+    plan->share_keys = a.chunk;
+    plan->shares = a.splits;
+    plan->launches = a.many ? 1 : (uint32_t)((a.units + a.each - 1) / a.each);
+    plan->workspace_bytes = a.ws_floats * sizeof(float);
+    return ok();
+}
 
 extern "C" int tc_cuda_paged_attention(tc_cuda_ctx *ctx, const tc_paged_cache *cache, const tc_paged_batch *batch,
                                        const tc_attention *attention, void *stream) {

@@ -118,6 +118,12 @@ class _Attention(C.Structure):
                 ("scale", C.c_float)]
 
 
+class AttentionPlan(C.Structure):
+    """struct tc_attention_plan."""
+    _fields_ = [("many_rows", _u32), ("rows", _u32), ("ctas_per_sm", _u32), ("share_keys", _u32), ("shares", _u32),
+                ("launches", _u32), ("workspace_bytes", _u64)]
+
+
 EXPORTS = {
     # name: (restype, argtypes)
     "tc_cuda_abi_version": (_u32, []),
@@ -181,6 +187,8 @@ EXPORTS = {
                                        C.c_float, C.POINTER(_Rope), _vp]),
     "tc_cuda_kv_append": (C.c_int, [_vp, C.POINTER(_PagedCache), C.POINTER(_PagedBatch), C.POINTER(_Heads),
                                     C.POINTER(_Heads), C.POINTER(_Heads), C.c_int, C.c_float, C.POINTER(_Rope), _vp]),
+    "tc_paged_attention_plan": (C.c_int, [_u32, _u32, _u32, _u32, _u32, C.POINTER(_PagedBatch), _i32, _i32,
+                                          C.POINTER(AttentionPlan)]),
     "tc_cuda_paged_attention": (C.c_int, [_vp, C.POINTER(_PagedCache), C.POINTER(_PagedBatch),
                                           C.POINTER(_Attention), _vp]),
 }
@@ -801,6 +809,19 @@ def paged_attention(ctx: Context, cache: PagedCache, batch: PagedBatch, q, scale
     batch.c.n_tokens = shape[0]
     _check(lib().tc_cuda_paged_attention(ctx.handle, cache.c, batch.c, a, _stream_of(ctx, stream)))
     return (out, lse) if return_lse else out
+
+
+def attention_plan(n_heads: int, cache_heads: int, head_dim: int, requests: int, tokens: int, max_new: int,
+                   max_length: int, causal: bool = True, window: int = 0, page_size: int = 16,
+                   table_width: int | None = None, sms: int = 148) -> AttentionPlan:
+    """How paged_attention divides a call of these sizes on a GPU of `sms` SMs
+    (tc_paged_attention_plan; needs no GPU)."""
+    b, plan = _PagedBatch(), AttentionPlan()
+    b.n_seq, b.n_tokens, b.max_new, b.max_length = requests, tokens, max_new, max_length
+    b.table_width = -(-max_length // page_size) if table_width is None else table_width
+    _check(lib().tc_paged_attention_plan(sms, n_heads, cache_heads, head_dim, page_size, b, causal,
+                                         min(max(window, -1), 2**31 - 1), plan))
+    return plan
 
 
 class GGUFError(BackendError):
