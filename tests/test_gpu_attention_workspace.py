@@ -1,0 +1,45 @@
+"""Paged attention where the GPU has no room for its partial results."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import attn_cases as ac
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("n,new,length,group,heads", [(1, 1536, 31537, 4, 8), (64, 1, 8000, 16, 8)])
+def test_a_full_gpu_costs_shares_not_the_call(n, new, length, group, heads):
+    """Many rows take one share, few rows go in smaller launches."""
+    from turbocider_b200 import cuda as tcc
+    g = ac.gen(71)
+    k, v, table, ks, vs = ac.paged([(new, length)], 64, heads, 128, torch.bfloat16, g)
+    offsets = torch.arange(n + 1, dtype=torch.int32, device="cuda") * new
+    lengths = torch.full((n,), length, dtype=torch.int32, device="cuda")
+    q = ac.normal(g, (n * new, heads * group, 128), torch.bfloat16)
+    args = tcc.PagedCache(k, v), tcc.PagedBatch(offsets, lengths, table.expand(n, -1).contiguous(), new, length), q
+    roomy, tight = tcc.Context(0), tcc.Context(0)
+    need = tcc.attention_plan(heads * group, heads, 128, n, n * new, new, length, page_size=64).workspace_bytes
+    assert need > 32 << 20
+    out = torch.empty_like(q)
+    want = tcc.paged_attention(roomy, *args)      # modules are loaded, and here is room
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    taken = torch.empty(torch.cuda.mem_get_info()[0] - need + (8 << 20), dtype=torch.uint8, device="cuda")
+    try:
+        for _ in range(2):
+            tcc.paged_attention(tight, *args, out=out)
+            torch.cuda.synchronize()
+        assert tight.status() == 0
+    finally:
+        del taken
+        torch.cuda.empty_cache()
+    # the same sums in another order: as far apart as two roundings of the probabilities and results
+    scale = vs[0].abs().max()
+    assert float((out.double() - want.double()).abs().max()) <= 4 * 2.0 ** -8 * float(scale)
+    tcc.paged_attention(tight, *args, out=out)    # room again
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    roomy.close()
+    tight.close()

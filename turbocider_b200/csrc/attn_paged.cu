@@ -575,30 +575,38 @@ bool encode_cache(CUtensorMap *map, const uint16_t *base, const CacheView &c, ui
 // (where one unit of work needs no more).
 constexpr uint64_t kWorkspaceMost = 256u << 20;
 
+// A fresh buffer of at least `need` bytes, `want` if there is room.
+cudaError_t grown(void **fresh, size_t &want, size_t need) {
+    cudaError_t e = cudaMalloc(fresh, want);
+    if (e != cudaSuccess && want > need) e = cudaMalloc(fresh, want = need);
+    if (e != cudaSuccess) cudaGetLastError();   // reported here, not by the next launch
+    return e;
+}
+
 // Grows the context's split workspace; the counters start at zero and every
 // complete kernel leaves them so.
 int ensure_split(tc_cuda_ctx *ctx, size_t floats, size_t counters, cudaStream_t s) {
     constexpr int room = sizeof(ctx->attn_outgrown) / sizeof(ctx->attn_outgrown[0]);
     if (floats > ctx->attn_ws_floats) {
         void *fresh = nullptr;
-        const size_t n = std::max(floats, 2 * ctx->attn_ws_floats);
+        size_t bytes = std::max(floats, 2 * ctx->attn_ws_floats) * sizeof(float);
         if (ctx->attn_outgrown_n == room) return fail("the attention workspace has grown too often");
-        const cudaError_t e = cudaMalloc(&fresh, n * sizeof(float));
+        const cudaError_t e = grown(&fresh, bytes, floats * sizeof(float));
         if (e != cudaSuccess) return cuda_fail("attention workspace allocation", e);
         if (ctx->attn_ws) ctx->attn_outgrown[ctx->attn_outgrown_n++] = ctx->attn_ws;
         ctx->attn_ws = static_cast<float *>(fresh);
-        ctx->attn_ws_floats = n;
+        ctx->attn_ws_floats = bytes / sizeof(float);
     }
     if (counters > ctx->attn_counters_n) {
         void *fresh = nullptr;
-        const size_t n = std::max(counters, 2 * ctx->attn_counters_n);
+        size_t bytes = std::max(counters, 2 * ctx->attn_counters_n) * sizeof(uint32_t);
         if (ctx->attn_outgrown_n == room) return fail("the attention workspace has grown too often");
-        cudaError_t e = cudaMalloc(&fresh, n * sizeof(uint32_t));
-        if (e == cudaSuccess && (e = cudaMemsetAsync(fresh, 0, n * sizeof(uint32_t), s)) != cudaSuccess) cudaFree(fresh);
+        cudaError_t e = grown(&fresh, bytes, counters * sizeof(uint32_t));
+        if (e == cudaSuccess && (e = cudaMemsetAsync(fresh, 0, bytes, s)) != cudaSuccess) cudaFree(fresh);
         if (e != cudaSuccess) return cuda_fail("attention counter allocation", e);
         if (ctx->attn_counters) ctx->attn_outgrown[ctx->attn_outgrown_n++] = ctx->attn_counters;
         ctx->attn_counters = static_cast<uint32_t *>(fresh);
-        ctx->attn_counters_n = n;
+        ctx->attn_counters_n = bytes / sizeof(uint32_t);
     }
     return TC_CUDA_OK;
 }
@@ -615,7 +623,7 @@ struct AttnPlan {
 };
 
 const char *plan_attention(const BatchView &bt, uint32_t n_kv, uint64_t group, uint32_t head_dim, uint32_t page_shift,
-                           bool causal, int32_t window, uint32_t sm_count, AttnPlan &a) {
+                           bool causal, int32_t window, uint32_t sm_count, uint64_t workspace_most, AttnPlan &a) {
     a = AttnPlan{};
     // longest span of keys one tile of rows sees (requests that their row of the
     // page table does not cover are not served)
@@ -635,17 +643,25 @@ const char *plan_attention(const BatchView &bt, uint32_t n_kv, uint64_t group, u
         a.n_blocks = (uint32_t)(rows / kChunkRows + bt.n_seq);
         // Shares of the keys: as many CTAs as make the busiest SM's work least,
         // in steps of 128 keys plus kCtaSteps for what a CTA does besides, one
-        // CTA per SM, and the time to join the shares (2 us and 0.5 us a share,
-        // in steps of 2 us); no share under kLeastSteps.
-        constexpr uint64_t kCtaSteps = 3, kLeastSteps = 2;
+        // CTA per SM, and the time to join the shares (2 us, 0.5 us a share, and
+        // their partial results written and read at 6.5 TB/s, all in quarters of
+        // a step of 2 us); no share under kLeastSteps, none for a gain of less than
+        // 1 in kLeastGain (a round more or less of thousands of CTAs is within the
+        // model's error, gigabytes of partial results are not), and no more than
+        // the workspace is to hold.
+        constexpr uint64_t kCtaSteps = 3, kLeastSteps = 2, kLeastGain = 32, kQuarterBytes = 3250000;
         const uint64_t steps = (span + kChunkKeys - 1) / kChunkKeys + 1;
         const uint64_t blocks = std::max<uint64_t>((rows + kChunkRows - 1) / kChunkRows, bt.n_seq);
-        uint64_t best = ~0ull, share = steps;
+        const uint64_t part_bytes = (uint64_t)n_kv * kChunkRows * (dp + 2) * sizeof(float);   // of a block and share
+        uint64_t one = 0, best = 0, share = steps;
         for (uint64_t n = 1; n <= kChunkShares && (n == 1 || steps / n >= kLeastSteps); ++n) {
             const uint64_t each = (steps + n - 1) / n, real = (steps + each - 1) / each;
+            if (real > 1 && a.n_blocks * real * part_bytes > workspace_most) break;
             const uint64_t waves = (blocks * n_kv * real + sm_count - 1) / sm_count;
-            const uint64_t cost = 4 * waves * (each + kCtaSteps) + (real > 1 ? 4 + real : 0);
-            if (cost < best) {
+            const uint64_t join = real > 1 ? 4 + real + 2 * blocks * real * part_bytes / kQuarterBytes : 0;
+            const uint64_t cost = 4 * waves * (each + kCtaSteps) + join;
+            if (n == 1) one = best = cost;
+            if (cost < best && cost + one / kLeastGain <= one) {
                 best = cost;
                 share = each;
             }
@@ -683,12 +699,12 @@ const char *plan_attention(const BatchView &bt, uint32_t n_kv, uint64_t group, u
     a.splits = (uint32_t)((span + chunk - 1) / chunk);
     a.ws_rows = (uint32_t)std::min<uint64_t>(rows_most, 16 * mt);
     // Units of a launch: a dimension of the grid, and no more than their partial
-    // results fit kWorkspaceMost bytes (at 16 KB or so a CTA that leaves tens of
+    // results fit the workspace (at 256 MB and 16 KB or so a CTA that leaves tens of
     // rounds over the GPU; launches on a stream take turns with the workspace).
     a.each = std::min<uint64_t>(a.units, 65535);
     if (a.splits > 1) {
         const uint64_t parts = (uint64_t)n_kv * a.splits * a.ws_rows;   // of a unit
-        a.each = std::max<uint64_t>(std::min(a.each, kWorkspaceMost / (parts * (dp + 2) * sizeof(float))), 1);
+        a.each = std::max<uint64_t>(std::min(a.each, workspace_most / (parts * (dp + 2) * sizeof(float))), 1);
         a.ws_ml = (a.each * parts * 2 + 3) / 4 * 4;
         a.ws_floats = a.ws_ml + a.each * parts * dp;
         a.counters = a.each * n_kv;
@@ -738,22 +754,24 @@ int attend(tc_cuda_ctx *ctx, const tc_paged_cache *cache, const tc_paged_batch *
     p.out_quads = !(reinterpret_cast<uintptr_t>(a->out) % 8) && !(a->ld_out_token % 4) && !(a->ld_out_head % 4);
     const bool bf16 = cache->dtype == TC_DTYPE_BF16;
 
+    CurrentDevice guard(ctx->device);
     AttnPlan plan;
-    if (const char *e = plan_attention(p.batch, c.n_heads, group, c.head_dim, c.page_shift, p.causal, p.window,
-                                       (uint32_t)ctx->sm_count, plan))
-        return fail(e);
+    for (uint64_t most = kWorkspaceMost;;) {
+        if (const char *e = plan_attention(p.batch, c.n_heads, group, c.head_dim, c.page_shift, p.causal, p.window,
+                                           (uint32_t)ctx->sm_count, most, plan))
+            return fail(e);
+        if (!plan.ws_floats || ensure_split(ctx, plan.ws_floats, plan.counters, s) == TC_CUDA_OK) break;
+        if (most != kWorkspaceMost) return TC_CUDA_FAIL;
+        most = std::min<uint64_t>(ctx->attn_ws_floats * sizeof(float), most - 1);   // no room: with what there is
+    }
     p.chunk = plan.chunk;
     p.splits = plan.splits;
     p.n_blocks = plan.n_blocks;
     p.row_tiles = plan.row_tiles;
     p.ws_rows = plan.ws_rows;
     p.ws_ml = plan.ws_ml;
-    CurrentDevice guard(ctx->device);
-    if (plan.ws_floats) {
-        if (ensure_split(ctx, plan.ws_floats, plan.counters, s)) return TC_CUDA_FAIL;
-        p.ws = ctx->attn_ws;
-        p.counters = ctx->attn_counters;
-    }
+    p.ws = ctx->attn_ws;
+    p.counters = ctx->attn_counters;
     const uint32_t dp = plan.dp, mt = plan.mt;
     const uint32_t keys = plan.many ? kChunkKeys : step_keys((int)dp, (int)mt);
     CUtensorMap km, vm;
@@ -808,7 +826,7 @@ extern "C" int tc_paged_attention_plan(uint32_t sm_count, uint32_t n_heads, uint
     if (group * bt.max_new > 0x7fffffffu) return fail("too many heads");
     AttnPlan a;
     if (const char *e = plan_attention(bt, cache_heads, group, head_dim, (uint32_t)__builtin_ctz(page_size), causal != 0,
-                                       std::min(window, kMaxLength), sm_count, a))
+                                       std::min(window, kMaxLength), sm_count, kWorkspaceMost, a))
         return fail(e);
     *plan = tc_attention_plan{};
     plan->many_rows = a.many;
