@@ -331,12 +331,13 @@ cudaError_t launch_sized(HeadsParams &p, bool half, bool wide, int sm_count, cud
     p.groups = (n_all + p.heads_per_group - 1) / p.heads_per_group;
     const uint64_t blocks = ((uint64_t)p.n_tokens * p.groups + kWarps - 1) / kWarps;
     if (blocks > 0x7fffffffu) return cudaErrorInvalidValue;
-    if (half) {
-        if (wide) heads_kernel<T, CH, true, APPEND, true><<<(unsigned)blocks, kWarps * 32, 0, s>>>(p);
-        else heads_kernel<T, CH, true, APPEND, false><<<(unsigned)blocks, kWarps * 32, 0, s>>>(p);
-    } else {
-        if (wide) heads_kernel<T, CH, false, APPEND, true><<<(unsigned)blocks, kWarps * 32, 0, s>>>(p);
-        else heads_kernel<T, CH, false, APPEND, false><<<(unsigned)blocks, kWarps * 32, 0, s>>>(p);
+    auto launch = [&](auto kernel) { kernel<<<(unsigned)blocks, kWarps * 32, 0, s>>>(p); };
+    if (wide) {
+        if (half) launch(heads_kernel<T, CH, true, APPEND, true>);
+        else launch(heads_kernel<T, CH, false, APPEND, true>);
+    } else if constexpr (CH == 4) {   // (chunks of 8 are taken only where they are aligned)
+        if (half) launch(heads_kernel<T, CH, true, APPEND, false>);
+        else launch(heads_kernel<T, CH, false, APPEND, false>);
     }
     return cudaGetLastError();
 }
