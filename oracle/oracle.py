@@ -34,6 +34,13 @@ _port = None
 _ref = None
 
 
+class ReferenceUnavailable(RuntimeError):
+    """The reference decoder was asked for and is not built here."""
+
+    def __init__(self):
+        super().__init__("reference decoder not built (oracle/_ref)")
+
+
 def build() -> None:
     """Build the port (always) and the reference decoder (when its sources exist)."""
     subprocess.run(["make", "-s", "-C", str(HERE)], check=True, capture_output=True)
@@ -96,7 +103,7 @@ def decode(raw, ggml_type: int, rows: int, cols: int, dtype: int = F32, which: s
     else:
         lib = ref()
         if lib is None:
-            raise RuntimeError("reference decoder not built (oracle/_ref)")
+            raise ReferenceUnavailable
         stats = (C.c_uint64 * 4)()
         rc = lib.tc_gguf_test_decode(*args, None, 0, 0, stats)
         err = lib.tc_gguf_test_error().decode()
@@ -118,7 +125,7 @@ def decode_gather(raw, ggml_type: int, rows: int, cols: int, indices, dtype: int
     if which == "ref":
         lib = ref()
         if lib is None:
-            raise RuntimeError("reference decoder not built (oracle/_ref)")
+            raise ReferenceUnavailable
         stats = (C.c_uint64 * 4)()
         rc = lib.tc_gguf_test_decode(ggml_type, src.ctypes.data, src.nbytes, rows, cols, 0, 0, col_begin, ncols,
                                      dtype, out.ctypes.data, out.nbytes, ncols * item, item,
@@ -151,6 +158,8 @@ def decode_parallel(raw, ggml_type: int, rows: int, cols: int, dtype: int = F32,
     """Row-split decode over host threads (as the reference's RowDecodePool,
     native/runtime/streaming/gguf_packed_bank.cpp:48-100).  ctypes releases the
     GIL during each call, so the threads run in parallel."""
+    if which == "ref" and ref() is None:
+        raise ReferenceUnavailable
     src = _as_u8(raw)
     threads = threads or os.cpu_count() or 1
     item = 4 if dtype == F32 else 2
