@@ -43,3 +43,32 @@ def test_a_full_gpu_costs_shares_not_the_call(n, new, length, group, heads):
     assert torch.equal(out, want)
     roomy.close()
     tight.close()
+
+
+@pytest.mark.parametrize("new,length", [(1536, 31537), (1, 9000)])
+def test_a_capture_that_would_have_to_grow_it_is_refused(new, length):
+    """With the reason (memory cannot be had in a capture), not by what the spoilt
+    capture does to the launch."""
+    from turbocider_b200 import cuda as tcc
+    rt = pytest.importorskip("cuda.bindings.runtime")
+    g = ac.gen(72)
+    k, v, table, ks, vs = ac.paged([(new, length)], 64, 2, 128, torch.bfloat16, g)
+    offsets, lengths = ac.offsets_of([(new, length)])
+    q = ac.normal(g, (new, 8, 128), torch.bfloat16)
+    args = tcc.PagedCache(k, v), tcc.PagedBatch(offsets, lengths, table, new, length), q
+    out, fresh, side = torch.empty_like(q), tcc.Context(0), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    err, = rt.cudaStreamBeginCapture(side.cuda_stream, rt.cudaStreamCaptureMode.cudaStreamCaptureModeGlobal)
+    assert err == rt.cudaError_t.cudaSuccess
+    try:
+        with pytest.raises(tcc.BackendError, match="attention workspace allocation.*captur"):
+            tcc.paged_attention(fresh, *args, out=out, stream=side)
+    finally:
+        rt.cudaStreamEndCapture(side.cuda_stream)
+        rt.cudaGetLastError()
+    tcc.paged_attention(fresh, *args, out=out, stream=side)   # outside it grows
+    torch.cuda.synchronize()
+    want, _, tol, _ = ac.attention_ref(q, [(new, length)], ks, vs, 128 ** -0.5, True, 0)
+    ac.close(out, want, tol)
+    assert fresh.status() == 0
+    fresh.close()

@@ -584,15 +584,15 @@ cudaError_t grown(void **fresh, size_t &want, size_t need) {
 }
 
 // Grows the context's split workspace; the counters start at zero and every
-// complete kernel leaves them so.
-int ensure_split(tc_cuda_ctx *ctx, size_t floats, size_t counters, cudaStream_t s) {
+// complete kernel leaves them so.  cudaErrorMemoryAllocation: no room.
+cudaError_t ensure_split(tc_cuda_ctx *ctx, size_t floats, size_t counters, cudaStream_t s) {
     constexpr int room = sizeof(ctx->attn_outgrown) / sizeof(ctx->attn_outgrown[0]);
     if (floats > ctx->attn_ws_floats) {
         void *fresh = nullptr;
         size_t bytes = std::max(floats, 2 * ctx->attn_ws_floats) * sizeof(float);
-        if (ctx->attn_outgrown_n == room) return fail("the attention workspace has grown too often");
+        if (ctx->attn_outgrown_n == room) return cudaErrorMemoryAllocation;   // grown too often
         const cudaError_t e = grown(&fresh, bytes, floats * sizeof(float));
-        if (e != cudaSuccess) return cuda_fail("attention workspace allocation", e);
+        if (e != cudaSuccess) return e;
         if (ctx->attn_ws) ctx->attn_outgrown[ctx->attn_outgrown_n++] = ctx->attn_ws;
         ctx->attn_ws = static_cast<float *>(fresh);
         ctx->attn_ws_floats = bytes / sizeof(float);
@@ -600,15 +600,15 @@ int ensure_split(tc_cuda_ctx *ctx, size_t floats, size_t counters, cudaStream_t 
     if (counters > ctx->attn_counters_n) {
         void *fresh = nullptr;
         size_t bytes = std::max(counters, 2 * ctx->attn_counters_n) * sizeof(uint32_t);
-        if (ctx->attn_outgrown_n == room) return fail("the attention workspace has grown too often");
+        if (ctx->attn_outgrown_n == room) return cudaErrorMemoryAllocation;
         cudaError_t e = grown(&fresh, bytes, counters * sizeof(uint32_t));
         if (e == cudaSuccess && (e = cudaMemsetAsync(fresh, 0, bytes, s)) != cudaSuccess) cudaFree(fresh);
-        if (e != cudaSuccess) return cuda_fail("attention counter allocation", e);
+        if (e != cudaSuccess) return e;
         if (ctx->attn_counters) ctx->attn_outgrown[ctx->attn_outgrown_n++] = ctx->attn_counters;
         ctx->attn_counters = static_cast<uint32_t *>(fresh);
         ctx->attn_counters_n = bytes / sizeof(uint32_t);
     }
-    return TC_CUDA_OK;
+    return cudaSuccess;
 }
 
 // How a call is divided over CTAs, by its sizes alone.
@@ -760,9 +760,11 @@ int attend(tc_cuda_ctx *ctx, const tc_paged_cache *cache, const tc_paged_batch *
         if (const char *e = plan_attention(p.batch, c.n_heads, group, c.head_dim, c.page_shift, p.causal, p.window,
                                            (uint32_t)ctx->sm_count, most, plan))
             return fail(e);
-        if (!plan.ws_floats || ensure_split(ctx, plan.ws_floats, plan.counters, s) == TC_CUDA_OK) break;
-        if (most != kWorkspaceMost) return TC_CUDA_FAIL;
-        most = std::min<uint64_t>(ctx->attn_ws_floats * sizeof(float), most - 1);   // no room: with what there is
+        const cudaError_t e = plan.ws_floats ? ensure_split(ctx, plan.ws_floats, plan.counters, s) : cudaSuccess;
+        if (e == cudaSuccess) break;
+        // no room: with what there is (any other error, as in a capture, is one)
+        if (e != cudaErrorMemoryAllocation || most != kWorkspaceMost) return cuda_fail("attention workspace allocation", e);
+        most = std::min<uint64_t>(ctx->attn_ws_floats * sizeof(float), most - 1);
     }
     p.chunk = plan.chunk;
     p.splits = plan.splits;
