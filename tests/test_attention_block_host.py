@@ -38,3 +38,9 @@ def test_inputs_that_the_projection_would_misread_are_refused(block, x):
 def test_an_input_elsewhere_is_refused(block):
     with pytest.raises(tcc.BackendError, match="context's device"):
         block(X, None)
+
+
+def test_a_step_without_tokens_is_empty(block):
+    block.ctx.device = -1   # where X is
+    y = block(X[:0], None)
+    assert y.shape == (0, HIDDEN) and y.dtype == torch.bfloat16

@@ -116,6 +116,8 @@ class AttentionBlock:
             raise tcc.BackendError(f"x must be a contiguous bf16 tensor [tokens, {self.qkv.k}]")
         if x.get_device() != self.ctx.device:
             raise tcc.BackendError("x must be on the context's device")
+        if not x.shape[0]:
+            return x.new_empty((0, self.out.n))
         caller = torch.cuda.current_stream(self.ctx.device)
         if stream is None:
             return self._run(x, batch, caller)
