@@ -71,3 +71,13 @@ def test_workspaces_stay_bounded(dim, heads, group):
                                                           (8, 4, 1536, 31537, 2)])
 def test_few_blocks_are_split(heads, group, new, length, least):
     assert tcc.attention_plan(heads * group, heads, 128, 1, new, new, length).shares >= least
+
+
+def test_shares_allow_for_uneven_lengths():
+    """Drafted tokens of several requests: a second round that only the longest
+    lengths would fill is no reason to split further (three shares of the window
+    take 20 us, five 28)."""
+    plan = tcc.attention_plan(20, 5, 64, 23, 23 * 4, 7, 6007, window=2048, page_size=32)
+    assert plan.rows == 32 and plan.shares == 3
+    # one request is as long as it is
+    assert tcc.attention_plan(64, 8, 64, 1, 4, 4, 20000).shares * 8 <= SMS * 2
