@@ -441,7 +441,9 @@ int tc_gguf_validate_split(const tc_gguf *const *shards, uint32_t n);
  * cache.  (The reference runs these as separate MLX array operations around
  * its linears, native/models/qwen21/transformer.cpp:857-953.)  All pointers
  * are device pointers; strides count elements; sums, norms, angles and the
- * softmax are fp32 or wider and every result is rounded once to its type.
+ * softmax's statistics are fp32 or wider and every result is rounded once to
+ * its type.  Attention also rounds the probabilities, between their sum and
+ * their product with the values, to the cache's 16-bit type.
  * Indices read from device memory (offsets, lengths, page numbers) are
  * checked there: an impossible one sets TC_STATUS_GEOMETRY and is skipped; the
  * keys and values of an impossible page count as zeros.

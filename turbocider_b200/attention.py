@@ -84,7 +84,7 @@ class PagePool:
 
 
 class AttentionBlock:
-    """Attention of one layer.  qkv: a Weight of (n_heads + 2 n_kv) head_dim
+    """Causal attention of one layer in bf16.  qkv: a Weight of (n_heads + 2 n_kv) head_dim
     rows (queries' heads, keys', values'); out: a Weight of n_heads head_dim
     columns.  q_norm / k_norm: f32 [head_dim], or None for no norm.  freq: the
     rotation's frequencies (cuda.rope_freqs), positions being the tokens' places

@@ -17,10 +17,12 @@ from pathlib import Path
 HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 OUT = HERE / "libturbocider_cuda.so"
-# The bounds-checked variant (-DTC_BOUNDS_CHECK): every output store, weight
-# chunk address and decode target offset is checked, an index outside sets
-# TC_STATUS_BOUNDS instead of faulting.  The substitute for compute-sanitizer
-# in the GPU tests; loaded when TURBOCIDER_CHECKED=1.
+# The bounds-checked variant (-DTC_BOUNDS_CHECK): in the linears and decoders
+# every output store, weight chunk address and decode target offset is checked,
+# an index outside sets TC_STATUS_BOUNDS instead of faulting (the attention
+# operators check what they read from device memory in both variants).  The
+# substitute for compute-sanitizer in the GPU tests; loaded when
+# TURBOCIDER_CHECKED=1.
 OUT_CHECKED = HERE / "libturbocider_cuda_checked.so"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = ["-std=c++17", "-O3", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall",

@@ -29,7 +29,7 @@
 // are split over CTAs: partial results (column-major, so that the 128 threads of
 // a tile store whole lines), which a second kernel joins in order.
 //
-// What bounds it (2 x 4224 image tokens, 30 heads of 128, f16; 493 us, 1111
+// What bounds it (2 x 4224 image tokens, 30 heads of 128, f16; 505 us, 1085
 // TFLOP/s, in the first milliseconds).  A step takes about 3340 cycles, and as
 // many with the exponentials left out: the tensor cores work through four
 // products of 128 x 64 keys, which take as long as 128 x 128 ones would (every
@@ -37,11 +37,11 @@
 // 128 x head_dim.  The special-function units are busy for 2048 of them (32768
 // exponentials).  Besides, a CTA costs about 8 us for finding its work, the
 // queries, the first product and the results.  In a loop the GPU's 1000 W cap
-// lowers the clock from 1965 to about 1700 MHz: 558 us (982 TFLOP/s, 72 % of
+// lowers the clock from 1965 to about 1700 MHz: 581 us (944 TFLOP/s, 69 % of
 // what cuBLAS sustains there).
 // Tried and dropped: one issuer and 128-key steps, where a tile waits for its
 // products (the same time on these, 2 % slower on prompts, 2 % faster on one long
-// chunk, 216 registers instead of 122); two threads per row; tiles taking turns
+// chunk, 216 registers instead of 119); two threads per row; tiles taking turns
 // with the special-function units; a quarter or an eighth of the exponentials by
 // polynomial (faster by 1 % at best, 7 % slower on the long chunk, where the
 // power cap binds most).

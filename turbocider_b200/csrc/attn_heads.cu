@@ -16,9 +16,10 @@
 // token's sines and cosines are formed once per warp, the norm's weights folded
 // into them, and the arithmetic is packed two fp32 to an operation: with 8-byte
 // chunks and plain arithmetic half of the time went into issuing instructions.
-// 8448 tokens x 60 heads of 128 (260 MB): 53 us, 4.9 TB/s; appending 281 MB:
-// 57.5 us.  More warps or heads in flight, batches read ahead, or a token split
-// over warps were each slower (52 to 79 us).
+// 8448 tokens x 60 heads of 128 (260 MB): 53.5 us, 4.9 TB/s; appending 281 MB:
+// 58.6 us.  Batches read ahead took 62 and 130 us, four warps a token with shared
+// sines and cosines 60 and 80 at best.  The limit of 80 registers (six blocks an
+// SM) costs five of the eight 8-element forms 4 to 16 bytes of spills a thread.
 //
 // The angle: freq / 2 pi is held as a 64-bit binary fraction of a turn and
 // multiplied by the position modulo 2^64, i.e. modulo one turn and exactly,

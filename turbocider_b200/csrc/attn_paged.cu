@@ -17,8 +17,8 @@
 // (partial outputs in the workspace, added in chunk order, so the result does
 // not depend on timing).
 //
-// A decode step of 96 requests, 1.5 GB of cache: 236 us, 6.48 TB/s (98.8 % of the
-// measured copy).  One token over 3001 positions (12 MB): 9.6 us, bound by one
+// A decode step of 96 requests, 1.5 GB of cache: 235 us, 6.52 TB/s (99 % of the
+// measured copy).  One token over 3001 positions (12 MB): 9.9 us, bound by one
 // CTA's chain: 0.9 us to its pages, 2 us to the first keys, 2 us of steps, 0.6 us to
 // join the warps, 1 us for the arrival, 1.5 us to add the shares.
 //
@@ -44,7 +44,8 @@ constexpr int step_keys(int dp, int mt) { return dp == 64 && mt <= 2 ? 32 : 16; 
 constexpr int kWarps = 4;
 constexpr uint32_t kMaxChunk = 1024;
 // CTAs that an SM has room for: by the rings for 16 rows (heads of 256 need 128 KB
-// for two stages), by the registers of 32 and 64 rows.
+// for two stages), by the registers of 32 and 64 rows (all 255 of them with 64,
+// where 256 bytes a thread spill).
 constexpr int ctas_per_sm(int dp, int mt) { return dp == 256 ? 1 : mt == 1 ? 3 : 2; }
 
 // Rows of a CTA: MT mma tiles of 16.
@@ -634,7 +635,18 @@ const char *plan_attention(const BatchView &bt, uint32_t n_kv, uint64_t group, u
     }
     const uint64_t rows_most = group * bt.max_new;
     // mma tiles of a CTA: all rows of a request in one CTA, so that K and V are
-    // read once, as far as the registers go.
+    // read once, as far as the registers go; beyond, blocks of 256 rows on the
+    // tensor cores.  This kernel against that one in us (caches cold, 4 cache heads):
+    //   rows a head       16     32     48-64  |  16     32     48-64   128
+    //                     head_dim 128         |  head_dim 64
+    //   1 x 500 keys     14/26  18/24   18/24  | 12/24  14/24   19/24   20/22
+    //   8 x 500          16/20  21/18   22/18  | 14/18  16/18   22/18   25/16
+    //   32 x 500         23/22  27/21   27/22  | 16/19  20/18   30/19   33/18
+    //   1 x 4000         20/32  27/32   27/33  | 16/28  20/28   29/28   31/28
+    //   8 x 4000         31/42  35/42   43/41  | 21/37  25/36   38/36   55/34
+    //   32 x 4000        70/74  80/72  135/74  | 43/70  49/66   99/68  182/53
+    // (48 to 64 rows of heads of 64 stay here for the few and short requests; many
+    // long ones would be faster there.)
     const uint32_t dp = a.dp = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
     const uint32_t mt = a.mt = rows_most <= 16 || dp == 256 ? 1 : rows_most <= 32 || dp == 128 ? 2 : 4;
     a.many = rows_most > mt * 16 && head_dim <= 128;

@@ -729,8 +729,9 @@ def qk_norm_rope(ctx: Context, q, k=None, rope: Rope | None = None, q_weight=Non
     """RMS norm over each head (eps None: no norm) and position rotation (rope
     None: none) of query and key heads [tokens, heads, head_dim] in one
     launch.  Weights: f32 [head_dim], the norm's (not read without one).
-    q_out / k_out may be q / k.  Returns (q_out, k_out).  Results that are not passed in come from the current
-    stream's memory: with another `stream`, pass them or order the two."""
+    q_out / k_out may be q / k.  Returns (q_out, k_out).  Results that are not
+    passed in come from the current stream's memory: with another `stream`,
+    pass them or order the two."""
     dtype, hk = _dtype_id(q), None
     device = ctx.device
     hq, q_out = _heads(device, q, q_out, q_weight, "q", True)
