@@ -486,41 +486,45 @@ extern "C" {
 int tc_rope_freqs(uint32_t rotary_dim, double theta, uint32_t scaling, double factor, double trained_length,
                   double beta_fast, double beta_slow, double *freq, float *amplitude) {
     using namespace tc;
-    if (!freq || !amplitude) return fail("null argument");
-    if (!rotary_dim || rotary_dim % 2) return fail("rotary_dim must be even");
-    if (!(theta > 0.0) || !std::isfinite(theta)) return fail("theta must be positive");
-    if (scaling > TC_ROPE_BANDS) return fail("unknown rotation scaling");
-    if (scaling != TC_ROPE_PLAIN && (!(factor >= 1.0) || !std::isfinite(factor))) return fail("factor must be at least 1");
-    if (scaling == TC_ROPE_NTK && rotary_dim <= 2) return fail("this scaling needs rotary_dim above 2");
-    if (scaling == TC_ROPE_YARN || scaling == TC_ROPE_BANDS) {
-        if (!(trained_length > 0.0) || !(beta_slow > 0.0) || !(beta_fast > beta_slow))
-            return fail("trained_length and beta_fast > beta_slow must be positive");
-        if (scaling == TC_ROPE_YARN && !(theta > 1.0)) return fail("this scaling needs theta above 1");
+    try {
+        if (!freq || !amplitude) return fail("null argument");
+        if (!rotary_dim || rotary_dim % 2) return fail("rotary_dim must be even");
+        if (!(theta > 0.0) || !std::isfinite(theta)) return fail("theta must be positive");
+        if (scaling > TC_ROPE_BANDS) return fail("unknown rotation scaling");
+        if (scaling != TC_ROPE_PLAIN && (!(factor >= 1.0) || !std::isfinite(factor))) return fail("factor must be at least 1");
+        if (scaling == TC_ROPE_NTK && rotary_dim <= 2) return fail("this scaling needs rotary_dim above 2");
+        if (scaling == TC_ROPE_YARN || scaling == TC_ROPE_BANDS) {
+            if (!(trained_length > 0.0) || !(beta_slow > 0.0) || !(beta_fast > beta_slow))
+                return fail("trained_length and beta_fast > beta_slow must be positive");
+            if (scaling == TC_ROPE_YARN && !(theta > 1.0)) return fail("this scaling needs theta above 1");
+        }
+        const double two_pi = 6.283185307179586476925, d = rotary_dim;
+        const uint32_t n = rotary_dim / 2;
+        if (scaling == TC_ROPE_NTK) theta *= std::pow(factor, d / (d - 2.0));
+        double low = 0.0, high = 0.0;
+        if (scaling == TC_ROPE_YARN) {
+            // pair index that turns beta times in trained_length
+            low = std::floor(d * std::log(trained_length / (beta_fast * two_pi)) / (2.0 * std::log(theta)));
+            high = std::ceil(d * std::log(trained_length / (beta_slow * two_pi)) / (2.0 * std::log(theta)));
+            low = low < 0.0 ? 0.0 : low;
+            high = high > d - 1.0 ? d - 1.0 : high;
+            if (high <= low) high = low + 0.001;
+        }
+        *amplitude = scaling == TC_ROPE_YARN ? (float)(0.1 * std::log(factor) + 1.0) : 1.f;
+        for (uint32_t i = 0; i < n; ++i) {
+            double f = std::pow(theta, -2.0 * i / d);
+            double keep = 1.0;   // share of the unscaled frequency
+            if (scaling == TC_ROPE_LINEAR) keep = 0.0;
+            if (scaling == TC_ROPE_YARN) keep = 1.0 - (i - low) / (high - low);
+            if (scaling == TC_ROPE_BANDS) keep = (trained_length * f / two_pi - beta_slow) / (beta_fast - beta_slow);
+            keep = keep < 0.0 ? 0.0 : keep > 1.0 ? 1.0 : keep;
+            if (scaling != TC_ROPE_PLAIN && scaling != TC_ROPE_NTK) f = f * keep + f / factor * (1.0 - keep);
+            freq[i] = f;
+        }
+        return ok();
+    } catch (...) {
+        return TC_CUDA_FAIL;
     }
-    const double two_pi = 6.283185307179586476925, d = rotary_dim;
-    const uint32_t n = rotary_dim / 2;
-    if (scaling == TC_ROPE_NTK) theta *= std::pow(factor, d / (d - 2.0));
-    double low = 0.0, high = 0.0;
-    if (scaling == TC_ROPE_YARN) {
-        // pair index that turns beta times in trained_length
-        low = std::floor(d * std::log(trained_length / (beta_fast * two_pi)) / (2.0 * std::log(theta)));
-        high = std::ceil(d * std::log(trained_length / (beta_slow * two_pi)) / (2.0 * std::log(theta)));
-        low = low < 0.0 ? 0.0 : low;
-        high = high > d - 1.0 ? d - 1.0 : high;
-        if (high <= low) high = low + 0.001;
-    }
-    *amplitude = scaling == TC_ROPE_YARN ? (float)(0.1 * std::log(factor) + 1.0) : 1.f;
-    for (uint32_t i = 0; i < n; ++i) {
-        double f = std::pow(theta, -2.0 * i / d);
-        double keep = 1.0;   // share of the unscaled frequency
-        if (scaling == TC_ROPE_LINEAR) keep = 0.0;
-        if (scaling == TC_ROPE_YARN) keep = 1.0 - (i - low) / (high - low);
-        if (scaling == TC_ROPE_BANDS) keep = (trained_length * f / two_pi - beta_slow) / (beta_fast - beta_slow);
-        keep = keep < 0.0 ? 0.0 : keep > 1.0 ? 1.0 : keep;
-        if (scaling != TC_ROPE_PLAIN && scaling != TC_ROPE_NTK) f = f * keep + f / factor * (1.0 - keep);
-        freq[i] = f;
-    }
-    return ok();
 }
 
 int tc_cuda_qk_norm_rope(tc_cuda_ctx *ctx, const tc_heads *q, const tc_heads *k, uint64_t n_tokens,

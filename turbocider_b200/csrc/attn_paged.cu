@@ -832,33 +832,37 @@ extern "C" int tc_paged_attention_plan(uint32_t sm_count, uint32_t n_heads, uint
                                        uint32_t page_size, const tc_paged_batch *batch, int32_t causal, int32_t window,
                                        tc_attention_plan *plan) {
     using namespace tc;
-    if (!batch || !plan) return fail("null argument");
-    if (!sm_count || !head_dim || head_dim % 8 || head_dim > 256 || !cache_heads || cache_heads > 65535 || !n_heads ||
-        n_heads % cache_heads || page_size < 8 || page_size > 65536 || (page_size & (page_size - 1)) || window < 0 ||
-        batch->max_length > (uint32_t)kMaxLength || !batch->n_seq || batch->n_seq > 0xffffffu || !batch->n_tokens ||
-        batch->n_tokens > 0x7fffffffu || !batch->max_new)
-        return fail("sizes that tc_cuda_paged_attention would not take");
-    BatchView bt{};
-    bt.n_seq = batch->n_seq;
-    bt.table_width = batch->table_width;
-    bt.n_tokens = batch->n_tokens;
-    bt.max_new = std::min(batch->max_new, batch->n_tokens);
-    bt.max_length = batch->max_length;
-    const uint64_t group = n_heads / cache_heads;
-    if (group * bt.max_new > 0x7fffffffu) return fail("too many heads");
-    AttnPlan a;
-    if (const char *e = plan_attention(bt, cache_heads, group, head_dim, (uint32_t)__builtin_ctz(page_size), causal != 0,
-                                       std::min(window, kMaxLength), sm_count, kWorkspaceMost, a))
-        return fail(e);
-    *plan = tc_attention_plan{};
-    plan->many_rows = a.many;
-    plan->rows = a.many ? kChunkRows : 16 * a.mt;
-    plan->ctas_per_sm = a.many ? 1 : (uint32_t)ctas_per_sm((int)a.dp, (int)a.mt);
-    plan->share_keys = a.chunk;
-    plan->shares = a.splits;
-    plan->launches = a.many ? 1 : (uint32_t)((a.units + a.each - 1) / a.each);
-    plan->workspace_bytes = a.ws_floats * sizeof(float);
-    return ok();
+    try {
+        if (!batch || !plan) return fail("null argument");
+        if (!sm_count || !head_dim || head_dim % 8 || head_dim > 256 || !cache_heads || cache_heads > 65535 || !n_heads ||
+            n_heads % cache_heads || page_size < 8 || page_size > 65536 || (page_size & (page_size - 1)) || window < 0 ||
+            batch->max_length > (uint32_t)kMaxLength || !batch->n_seq || batch->n_seq > 0xffffffu || !batch->n_tokens ||
+            batch->n_tokens > 0x7fffffffu || !batch->max_new)
+            return fail("sizes that tc_cuda_paged_attention would not take");
+        BatchView bt{};
+        bt.n_seq = batch->n_seq;
+        bt.table_width = batch->table_width;
+        bt.n_tokens = batch->n_tokens;
+        bt.max_new = std::min(batch->max_new, batch->n_tokens);
+        bt.max_length = batch->max_length;
+        const uint64_t group = n_heads / cache_heads;
+        if (group * bt.max_new > 0x7fffffffu) return fail("too many heads");
+        AttnPlan a;
+        if (const char *e = plan_attention(bt, cache_heads, group, head_dim, (uint32_t)__builtin_ctz(page_size), causal != 0,
+                                           std::min(window, kMaxLength), sm_count, kWorkspaceMost, a))
+            return fail(e);
+        *plan = tc_attention_plan{};
+        plan->many_rows = a.many;
+        plan->rows = a.many ? kChunkRows : 16 * a.mt;
+        plan->ctas_per_sm = a.many ? 1 : (uint32_t)ctas_per_sm((int)a.dp, (int)a.mt);
+        plan->share_keys = a.chunk;
+        plan->shares = a.splits;
+        plan->launches = a.many ? 1 : (uint32_t)((a.units + a.each - 1) / a.each);
+        plan->workspace_bytes = a.ws_floats * sizeof(float);
+        return ok();
+    } catch (...) {
+        return TC_CUDA_FAIL;
+    }
 }
 
 extern "C" int tc_cuda_paged_attention(tc_cuda_ctx *ctx, const tc_paged_cache *cache, const tc_paged_batch *batch,
