@@ -49,8 +49,8 @@ def test_no_gigabytes_for_a_rounding_of_the_rounds():
 @pytest.mark.parametrize("heads,group", [(1, 1), (1, 32), (2, 8), (8, 4), (8, 8), (30, 1), (64, 1)])
 def test_workspaces_stay_bounded(dim, heads, group):
     """Partial results: never more than 256 MB but for a single request whose one
-    tile of rows over its whole cache needs more; never more than a quarter of
-    what the call reads and computes is worth."""
+    tile of rows over its whole cache needs more; many rows' take no longer to
+    move than the call's products, or 40 us."""
     for requests in (1, 2, 3, 7, 16, 64, 200, 1000):
         for new in (1, 2, 5, 16, 40, 100, 333, 1000, 4096, 8192):
             for past in (0, 500, 4000, 30000, 262144, 10 ** 6):
